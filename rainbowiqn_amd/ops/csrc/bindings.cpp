@@ -578,7 +578,10 @@ void heads_gemm_fp8(torch::Tensor hq, torch::Tensor hsc, torch::Tensor wq,
 
 }  // namespace
 
+void bind_blocks(py::module& m);  // bindings_blocks.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    bind_blocks(m);
     m.def("replay_append", &replay_append);
     m.def("replay_sample", &replay_sample);
     m.def("replay_update_priorities", &replay_update_priorities);

@@ -1,0 +1,527 @@
+// Torch bindings of the 8-bit block matrices and of layer norm.  Each function
+// is one direction of an operator: it checks its arguments, allocates outputs
+// and workspaces from torch's caching allocator (so they are safe in captured
+// graphs) and launches on the current stream of the arguments' device.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <hip/hip_runtime_api.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <tuple>
+
+#include "riqn_kernels.h"
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+void* stream_of(const Tensor& t) {
+    return (void*)at::cuda::getCurrentCUDAStream(t.device().index()).stream();
+}
+
+void launched(int err, const char* what) {
+    TORCH_CHECK(err == 0, what, ": ", hipGetErrorString((hipError_t)err));
+}
+
+int type_code(at::ScalarType t, const char* name) {
+    switch (t) {
+        case torch::kFloat32: return 0;
+        case torch::kBFloat16: return 1;
+        case torch::kFloat16: return 2;
+        default:
+            TORCH_CHECK(false, name, " must be float32, bfloat16 or float16, got ",
+                        at::toString(t));
+    }
+}
+
+// a matrix whose rows are contiguous and any stride apart
+void check_rows(const Tensor& x, const char* name) {
+    TORCH_CHECK(x.is_cuda(), name, " must be on GPU");
+    TORCH_CHECK(x.dim() == 2, name, " must have 2 dimensions");
+    TORCH_CHECK(x.size(1) <= 1 || x.stride(1) == 1 || x.numel() == 0, name,
+                " must have contiguous rows");
+    TORCH_CHECK(x.size(0) <= (1 << 30) && x.size(1) <= (1 << 24), name,
+                " must have at most 2^30 rows and 2^24 columns");
+}
+
+void check_vector(const Tensor& v, int64_t n, const Tensor& like,
+                  const char* name) {
+    TORCH_CHECK(v.device() == like.device(), name, " must be on ", like.device());
+    TORCH_CHECK(v.dim() == 1 && v.size(0) == n, name, " must have ", n,
+                " elements in 1 dimension");
+    TORCH_CHECK(v.is_contiguous(), name, " must be contiguous");
+}
+
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+int64_t padded4(int64_t n) { return (n + 3) / 4 * 4; }
+
+struct Blocks {
+    Tensor q, scale;
+    int64_t rows, block_rows;
+};
+
+// checks what the kernels take for granted about a matrix given from outside
+Blocks check_blocks(const Tensor& q, const Tensor& scale, int64_t cols,
+                    int64_t block_rows, const char* name) {
+    TORCH_CHECK(q.is_cuda() && scale.device() == q.device(), name,
+                ": q and scale must be on one GPU");
+    TORCH_CHECK(q.scalar_type() == torch::kUInt8 &&
+                    scale.scalar_type() == torch::kUInt8,
+                name, ": q and scale must be uint8");
+    TORCH_CHECK(block_rows == 1 || block_rows == 128, name,
+                ": block_rows must be 1 or 128");
+    TORCH_CHECK(cols >= 1 && cols <= (1 << 24), name,
+                ": must have 1 to 2^24 columns");
+    const int64_t nb = blocks_of(cols);
+    TORCH_CHECK(q.dim() == 2 && q.size(1) == nb * 128 && q.is_contiguous(),
+                name, ": q must be contiguous [rows, ", nb * 128, "]");
+    TORCH_CHECK(q.size(0) <= (1 << 30), name, ": must have at most 2^30 rows");
+    const int64_t sr =
+        block_rows == 1 ? q.size(0) : (q.size(0) + 127) / 128;
+    TORCH_CHECK(scale.dim() == 2 && scale.size(0) == sr &&
+                    scale.size(1) == padded4(nb) && scale.is_contiguous(),
+                name, ": scale must be contiguous [", sr, ", ", padded4(nb), "]");
+    TORCH_CHECK(((uintptr_t)q.data_ptr() & 15) == 0 &&
+                    ((uintptr_t)scale.data_ptr() & 3) == 0,
+                name, ": q must be 16-byte and scale 4-byte aligned");
+    return {q, scale, q.size(0), block_rows};
+}
+
+at::TensorOptions bytes_on(const Tensor& t) {
+    return t.options().dtype(torch::kUInt8);
+}
+at::TensorOptions floats_on(const Tensor& t) {
+    return t.options().dtype(torch::kFloat32);
+}
+
+// Workgroups that share out the rows: one for each pass of `rows_per_pass`
+// rows, at most `most`.
+int row_groups(int64_t rows, int64_t rows_per_pass, int64_t most) {
+    return (int)std::min<int64_t>((rows + rows_per_pass - 1) / rows_per_pass,
+                                  most);
+}
+
+// scale per 1 x 128 block; with `mask` values whose bit is clear count as
+// zero; `sum` (may be undefined) gets the sums of the columns
+Blocks quant_rows(const Tensor& x, const uint8_t* mask, Tensor* sum) {
+    const int64_t R = x.size(0), C = x.size(1), nb = blocks_of(C);
+    Blocks o{torch::empty({R, nb * 128}, bytes_on(x)),
+             torch::empty({R, padded4(nb)}, bytes_on(x)), R, 1};
+    const bool wide = nb >= 4;
+    const int64_t strips = wide ? (nb + 3) / 4 : nb;
+    // every group leaves a row of partial sums to be added up: 1024
+    // workgroups in all fill the card and keep those few
+    const int groups =
+        row_groups(R, wide ? 4 : 16,
+                   sum ? std::max<int64_t>(1, 1024 / strips) : 65535);
+    Tensor part;
+    if (sum) part = torch::empty({groups, C}, floats_on(x));
+    const int type = type_code(x.scalar_type(), "x");
+    launched(riqn_fp8_quant_rows(
+                 x.data_ptr(), type, x.stride(0), mask,
+                 o.q.data_ptr<uint8_t>(), o.scale.data_ptr<uint8_t>(),
+                 sum ? part.data_ptr<float>() : nullptr, groups, (int)R,
+                 (int)C, stream_of(x)),
+             "quantize_fp8_blocks");
+    if (sum)
+        launched(riqn_column_sum(part.data_ptr<float>(), sum->data_ptr(),
+                                 type_code(sum->scalar_type(), "bias"), groups,
+                                 (int)C, stream_of(x)),
+                 "column sum");
+    return o;
+}
+
+// scale per 128 x 128 block, and the transposed matrix where `t` is given
+Blocks quant_tiles(const Tensor& x, Blocks* t) {
+    const int64_t R = x.size(0), C = x.size(1);
+    const int64_t nb = blocks_of(C), nbt = blocks_of(R);
+    TORCH_CHECK(nbt <= 65535, "a matrix with a scale per 128 x 128 block must "
+                "have at most 65535 blocks of rows");
+    Blocks o{torch::empty({R, nb * 128}, bytes_on(x)),
+             torch::empty({nbt, padded4(nb)}, bytes_on(x)), R, 128};
+    if (t)
+        *t = Blocks{torch::empty({C, nbt * 128}, bytes_on(x)),
+                    torch::empty({nb, padded4(nbt)}, bytes_on(x)), C, 128};
+    launched(riqn_fp8_quant_tiles(
+                 x.data_ptr(), type_code(x.scalar_type(), "x"), x.stride(0),
+                 o.q.data_ptr<uint8_t>(), o.scale.data_ptr<uint8_t>(),
+                 t ? t->q.data_ptr<uint8_t>() : nullptr,
+                 t ? t->scale.data_ptr<uint8_t>() : nullptr, (int)R, (int)C,
+                 stream_of(x)),
+             "quantize_fp8_blocks");
+    return o;
+}
+
+void gemm(const Blocks& a, const Blocks& b, int64_t K, const OptTensor& bias,
+          bool relu, Tensor& c, uint8_t* mask) {
+    launched(riqn_fp8_gemm(
+                 a.q.data_ptr<uint8_t>(), a.scale.data_ptr<uint8_t>(),
+                 (int)a.block_rows, b.q.data_ptr<uint8_t>(),
+                 b.scale.data_ptr<uint8_t>(), (int)b.block_rows,
+                 bias ? bias->data_ptr() : nullptr,
+                 bias ? type_code(bias->scalar_type(), "bias") : 0, relu,
+                 c.data_ptr(), type_code(c.scalar_type(), "out"), mask,
+                 (int)a.rows, (int)b.rows, (int)K, stream_of(c)),
+             "matmul_fp8_blocks");
+}
+
+std::tuple<Tensor, Tensor> fp8_blocks_quant(Tensor x, int64_t block_rows) {
+    check_rows(x, "x");
+    TORCH_CHECK(x.size(1) >= 1, "x must have at least one column");
+    TORCH_CHECK(block_rows == 1 || block_rows == 128, "block_rows must be 1 or 128");
+    type_code(x.scalar_type(), "x");
+    c10::cuda::CUDAGuard guard(x.device());
+    if (x.size(0) == 0) {
+        const int64_t nb = blocks_of(x.size(1));
+        return {torch::empty({0, nb * 128}, bytes_on(x)),
+                torch::empty({0, padded4(nb)}, bytes_on(x))};
+    }
+    Blocks o = block_rows == 1 ? quant_rows(x, nullptr, nullptr)
+                               : quant_tiles(x, nullptr);
+    return {o.q, o.scale};
+}
+
+Tensor fp8_blocks_dequant(Tensor q, Tensor scale, int64_t cols,
+                          int64_t block_rows, at::ScalarType dtype) {
+    Blocks b = check_blocks(q, scale, cols, block_rows, "blocks");
+    const int type = type_code(dtype, "dtype");
+    c10::cuda::CUDAGuard guard(q.device());
+    Tensor out = torch::empty({b.rows, cols}, q.options().dtype(dtype));
+    if (b.rows == 0) return out;
+    launched(riqn_fp8_dequant(q.data_ptr<uint8_t>(), scale.data_ptr<uint8_t>(),
+                              out.data_ptr(), type, (int)b.rows, (int)cols,
+                              block_rows == 128 ? 7 : 0, stream_of(q)),
+             "dequantize_fp8_blocks");
+    return out;
+}
+
+Tensor fp8_blocks_matmul(Tensor aq, Tensor as, int64_t a_block_rows, Tensor bq,
+                         Tensor bs, int64_t b_block_rows, int64_t cols,
+                         OptTensor bias, bool relu, at::ScalarType dtype) {
+    Blocks a = check_blocks(aq, as, cols, a_block_rows, "a");
+    Blocks b = check_blocks(bq, bs, cols, b_block_rows, "b");
+    TORCH_CHECK(aq.device() == bq.device(), "a and b must be on one GPU");
+    if (bias) {
+        check_vector(*bias, b.rows, aq, "bias");
+        type_code(bias->scalar_type(), "bias");
+    }
+    type_code(dtype, "out_dtype");
+    c10::cuda::CUDAGuard guard(aq.device());
+    Tensor c = torch::empty({a.rows, b.rows}, aq.options().dtype(dtype));
+    if (c.numel() == 0) return c;
+    gemm(a, b, cols, bias, relu, c, nullptr);
+    return c;
+}
+
+// x [..., C] as a matrix of contiguous rows, copied only where it must
+Tensor as_rows(const Tensor& x) {
+    Tensor r = x;
+    if (x.dim() != 2) {
+        TORCH_CHECK(x.dim() > 0, "a matrix or a vector is wanted, not a number");
+        const int64_t c = x.size(-1);
+        r = x.reshape({x.numel() / std::max<int64_t>(1, c), c});
+    }
+    return r.size(1) <= 1 || r.stride(1) == 1 ? r : r.contiguous();
+}
+
+std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
+    auto s = x.sizes().vec();
+    s.back() = n;
+    return s;
+}
+
+bool wants_grad(const Tensor& t) { return t.requires_grad(); }
+bool wants_grad(const OptTensor& t) { return t && t->requires_grad(); }
+
+// Gradients whose own gradients are not there: where a graph of the backward
+// pass is being built, its use raises instead of counting as zero.
+torch::autograd::variable_list once(torch::autograd::variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    torch::autograd::variable_list fake;
+    for (auto& g : grads)
+        fake.push_back(g.defined() ? g.detach().set_requires_grad(true) : g);
+    auto err = std::make_shared<torch::autograd::DelayedError>(
+        "this operator is differentiable once", (int)fake.size());
+    return (*err)(std::move(fake));
+}
+
+struct LinearSaved {
+    Tensor xq, xs;                // x in 8 bits
+    Tensor wtq, wts;              // W transposed in 8 bits, for dx
+    Tensor bits;                  // the relu's
+};
+
+// y = x W^T + bias, relu; `keep` gets what the backward pass reads
+Tensor linear_fwd(const Tensor& x, const Tensor& w, const OptTensor& bias,
+                  bool relu, bool need_dx, LinearSaved* keep) {
+    check_rows(x, "x");
+    check_rows(w, "weight");
+    TORCH_CHECK(w.device() == x.device(), "weight must be on ", x.device());
+    TORCH_CHECK(x.size(1) >= 1 && x.size(1) == w.size(1), "x has ", x.size(1),
+                " columns and weight ", w.size(1));
+    TORCH_CHECK(w.size(0) >= 1, "weight must have at least one row");
+    if (bias) {
+        check_vector(*bias, w.size(0), x, "bias");
+        type_code(bias->scalar_type(), "bias");
+    }
+    type_code(x.scalar_type(), "x");
+    type_code(w.scalar_type(), "weight");
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t M = x.size(0), N = w.size(0), K = x.size(1);
+    Tensor y = torch::empty({M, N}, x.options());
+    if (M == 0 && !keep) return y;
+    Blocks wt;
+    Blocks wq = quant_tiles(w, need_dx ? &wt : nullptr);
+    Tensor bits;
+    if (relu && keep)
+        bits = torch::empty({M, blocks_of(N) * 16}, bytes_on(x));
+    Blocks xq;
+    if (M > 0) {
+        xq = quant_rows(x, nullptr, nullptr);
+        gemm(xq, wq, K, bias, relu, y,
+             bits.defined() ? bits.data_ptr<uint8_t>() : nullptr);
+    } else {
+        xq = {torch::empty({0, blocks_of(K) * 128}, bytes_on(x)),
+              torch::empty({0, padded4(blocks_of(K))}, bytes_on(x)), 0, 1};
+    }
+    if (keep) *keep = {xq.q, xq.scale, wt.q, wt.scale, bits};
+    return y;
+}
+
+struct LinearGrads {
+    Tensor dx, dw, db;
+};
+
+// each gradient only where its dtype is given
+LinearGrads linear_bwd(const Tensor& dy, const LinearSaved& s, int64_t K,
+                       c10::optional<at::ScalarType> dx_type,
+                       c10::optional<at::ScalarType> dw_type,
+                       c10::optional<at::ScalarType> db_type) {
+    check_rows(dy, "dy");
+    type_code(dy.scalar_type(), "dy");
+    const int64_t M = dy.size(0), N = dy.size(1);
+    TORCH_CHECK(s.xq.size(0) == M, "dy has ", M, " rows and x ", s.xq.size(0));
+    c10::cuda::CUDAGuard guard(dy.device());
+    LinearGrads o;
+    if (dx_type) o.dx = torch::empty({M, K}, dy.options().dtype(*dx_type));
+    if (dw_type) o.dw = torch::empty({N, K}, dy.options().dtype(*dw_type));
+    if (db_type) o.db = torch::empty({N}, dy.options().dtype(*db_type));
+    if (M == 0) {
+        if (dw_type) o.dw.zero_();
+        if (db_type) o.db.zero_();
+        return o;
+    }
+    Blocks g = quant_rows(
+        dy, s.bits.defined() ? s.bits.data_ptr<uint8_t>() : nullptr,
+        db_type ? &o.db : nullptr);
+    if (dx_type) {
+        Blocks wt{s.wtq, s.wts, K, 128};
+        gemm(g, wt, N, c10::nullopt, false, o.dx, nullptr);
+    }
+    if (dw_type) {
+        // a share of the rows for each workgroup of a tile: enough for two
+        // workgroups a CU, and at least 256 rows each
+        const int64_t tiles = blocks_of(N) * blocks_of(K);
+        const int shares = (int)std::max<int64_t>(
+            1, std::min<int64_t>(std::min<int64_t>(512 / tiles, M / 256), 64));
+        Tensor part;
+        if (shares > 1) part = torch::empty({shares, N, K}, floats_on(dy));
+        launched(riqn_fp8_wgrad(
+                     g.q.data_ptr<uint8_t>(), g.scale.data_ptr<uint8_t>(),
+                     s.xq.data_ptr<uint8_t>(), s.xs.data_ptr<uint8_t>(),
+                     o.dw.data_ptr(), type_code(*dw_type, "weight"),
+                     shares > 1 ? part.data_ptr<float>() : nullptr, shares,
+                     (int)M, (int)N, (int)K, stream_of(dy)),
+                 "linear_fp8_blocks backward");
+    }
+    return o;
+}
+
+// Autograd in C++: a training step of a small batch is bound by the host, and
+// a Python autograd function costs more than its kernels.
+class LinearFn : public torch::autograd::Function<LinearFn> {
+  public:
+    static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor x,
+                          Tensor w, OptTensor bias, bool relu, bool ndx,
+                          bool ndw, bool ndb) {
+        const Tensor x2 = as_rows(x);
+        LinearSaved s;
+        Tensor y = linear_fwd(x2, as_rows(w), bias, relu, ndx, &s);
+        ctx->save_for_backward({s.xq, s.xs, s.wtq, s.wts, s.bits});
+        auto& d = ctx->saved_data;
+        d["shape"] = x.sizes().vec();
+        d["dx"] = ndx ? (int64_t)x.scalar_type() : -1;
+        d["dw"] = ndw ? (int64_t)w.scalar_type() : -1;
+        d["db"] = ndb ? (int64_t)bias->scalar_type() : -1;
+        return y.view(with_last(x, w.size(0)));
+    }
+    static torch::autograd::variable_list backward(
+        torch::autograd::AutogradContext* ctx,
+        torch::autograd::variable_list dy) {
+        const auto v = ctx->get_saved_variables();
+        auto& d = ctx->saved_data;
+        const auto shape = d["shape"].toIntVector();
+        auto type = [&](const char* n) -> c10::optional<at::ScalarType> {
+            const int64_t t = d[n].toInt();
+            if (t < 0) return c10::nullopt;
+            return (at::ScalarType)t;
+        };
+        LinearGrads g = linear_bwd(as_rows(dy[0]), {v[0], v[1], v[2], v[3], v[4]},
+                                   shape.back(), type("dx"), type("dw"),
+                                   type("db"));
+        if (g.dx.defined()) g.dx = g.dx.view(shape);
+        return once({g.dx, g.dw, g.db, Tensor(), Tensor(), Tensor(), Tensor()});
+    }
+};
+
+Tensor linear_fp8(Tensor x, Tensor w, OptTensor bias, bool relu) {
+    TORCH_CHECK(w.dim() == 2, "weight must have 2 dimensions");
+    if (!at::GradMode::is_enabled() ||
+        !(wants_grad(x) || wants_grad(w) || wants_grad(bias)))
+        return linear_fwd(as_rows(x), as_rows(w), bias, relu, false, nullptr)
+            .view(with_last(x, w.size(0)));
+    return LinearFn::apply(x, w, bias, relu, wants_grad(x), wants_grad(w),
+                           wants_grad(bias));
+}
+
+// the same against a weight that is in 8 bits already; no gradients
+Tensor linear_fp8_serve(Tensor x0, Tensor wq, Tensor ws, int64_t block_rows,
+                        OptTensor bias, bool relu) {
+    TORCH_CHECK(!at::GradMode::is_enabled() ||
+                    !(wants_grad(x0) || wants_grad(bias)),
+                "a weight in 8-bit blocks is for serving: pass the float "
+                "weight where gradients are wanted");
+    const Tensor x = as_rows(x0);
+    check_rows(x, "x");
+    Blocks w = check_blocks(wq, ws, x.size(1), block_rows, "weight");
+    TORCH_CHECK(wq.device() == x.device(), "weight must be on ", x.device());
+    if (bias) {
+        check_vector(*bias, w.rows, x, "bias");
+        type_code(bias->scalar_type(), "bias");
+    }
+    type_code(x.scalar_type(), "x");
+    c10::cuda::CUDAGuard guard(x.device());
+    Tensor y = torch::empty({x.size(0), w.rows}, x.options());
+    if (y.numel() > 0)
+        gemm(quant_rows(x, nullptr, nullptr), w, x.size(1), bias, relu, y,
+             nullptr);
+    return y.view(with_last(x0, w.rows));
+}
+
+int norm_weights(const Tensor& x, const OptTensor& w, const OptTensor& b) {
+    const int xt = type_code(x.scalar_type(), "x");
+    int wt = -1;
+    for (const auto* t : {&w, &b}) {
+        if (!*t) continue;
+        check_vector(**t, x.size(1), x, "weight and bias");
+        const int code = type_code((*t)->scalar_type(), "weight and bias");
+        TORCH_CHECK(code == xt || code == 0,
+                    "weight and bias must have x's dtype or float32");
+        TORCH_CHECK(wt < 0 || wt == code, "weight and bias must have one dtype");
+        wt = code;
+    }
+    return wt < 0 ? xt : wt;
+}
+
+// mean and rstd: null where no backward pass will ask for them
+Tensor norm_fwd(const Tensor& x, const OptTensor& w, const OptTensor& b,
+                double eps, Tensor* mean, Tensor* rstd) {
+    check_rows(x, "x");
+    TORCH_CHECK(x.size(1) >= 1, "x must have at least one column");
+    TORCH_CHECK(eps >= 0.0, "eps must not be negative");
+    const int wt = norm_weights(x, w, b);
+    c10::cuda::CUDAGuard guard(x.device());
+    Tensor y = torch::empty({x.size(0), x.size(1)}, x.options());
+    if (mean) {
+        *mean = torch::empty({x.size(0)}, floats_on(x));
+        *rstd = torch::empty({x.size(0)}, floats_on(x));
+    }
+    if (x.size(0) > 0)
+        launched(riqn_norm_fwd(
+                     x.data_ptr(), type_code(x.scalar_type(), "x"), x.stride(0),
+                     w ? w->data_ptr() : nullptr, b ? b->data_ptr() : nullptr,
+                     wt, y.data_ptr(), mean ? mean->data_ptr<float>() : nullptr,
+                     rstd ? rstd->data_ptr<float>() : nullptr, (int)x.size(0),
+                     (int)x.size(1), (float)eps, stream_of(x)),
+                 "layer_norm");
+    return y;
+}
+
+class NormFn : public torch::autograd::Function<NormFn> {
+  public:
+    static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor x,
+                          OptTensor w, OptTensor b, double eps, bool ndx,
+                          bool ndw, bool ndb) {
+        const Tensor x2 = as_rows(x);
+        Tensor mean, rstd;
+        Tensor y = norm_fwd(x2, w, b, eps, &mean, &rstd);
+        ctx->save_for_backward({x2, w ? *w : Tensor(), mean, rstd});
+        auto& d = ctx->saved_data;
+        d["shape"] = x.sizes().vec();
+        d["wtype"] = (int64_t)(w ? *w : b ? *b : x).scalar_type();
+        d["need"] = (int64_t)(ndx | ndw << 1 | ndb << 2);
+        return y.view(x.sizes());
+    }
+    static torch::autograd::variable_list backward(
+        torch::autograd::AutogradContext* ctx,
+        torch::autograd::variable_list grad) {
+        const auto v = ctx->get_saved_variables();
+        const Tensor &x = v[0], &w = v[1], &mean = v[2], &rstd = v[3];
+        auto& d = ctx->saved_data;
+        const int64_t need = d["need"].toInt();
+        const auto w_type = (at::ScalarType)d["wtype"].toInt();
+        const Tensor dy = as_rows(grad[0]);
+        TORCH_CHECK(dy.sizes() == x.sizes() && dy.device() == x.device() &&
+                        dy.scalar_type() == x.scalar_type(),
+                    "dy must have x's shape, device and dtype");
+        const int64_t R = x.size(0), C = x.size(1);
+        c10::cuda::CUDAGuard guard(x.device());
+        Tensor dx, dw, db;
+        if (need & 1) dx = torch::empty({R, C}, x.options());
+        if (need & 2) dw = torch::empty({C}, x.options().dtype(w_type));
+        if (need & 4) db = torch::empty({C}, x.options().dtype(w_type));
+        if (R == 0) {
+            if (dw.defined()) dw.zero_();
+            if (db.defined()) db.zero_();
+        } else {
+            const int groups = row_groups(R, 4, 512);
+            Tensor part;
+            if (need & 6) part = torch::empty({groups, 2, C}, floats_on(x));
+            launched(riqn_norm_bwd(
+                         dy.data_ptr(), x.data_ptr(),
+                         type_code(x.scalar_type(), "x"), dy.stride(0),
+                         x.stride(0), w.defined() ? w.data_ptr() : nullptr,
+                         type_code(w_type, "weight"), mean.data_ptr<float>(),
+                         rstd.data_ptr<float>(),
+                         need & 1 ? dx.data_ptr() : nullptr,
+                         need & 2 ? dw.data_ptr() : nullptr,
+                         need & 4 ? db.data_ptr() : nullptr,
+                         need & 6 ? part.data_ptr<float>() : nullptr, groups,
+                         (int)R, (int)C, stream_of(x)),
+                     "layer_norm backward");
+        }
+        if (need & 1) dx = dx.view(d["shape"].toIntVector());
+        return once({dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()});
+    }
+};
+
+Tensor layer_norm(Tensor x, OptTensor w, OptTensor b, double eps) {
+    if (!at::GradMode::is_enabled() ||
+        !(wants_grad(x) || wants_grad(w) || wants_grad(b)))
+        return norm_fwd(as_rows(x), w, b, eps, nullptr, nullptr)
+            .view(x.sizes());
+    return NormFn::apply(x, w, b, eps, wants_grad(x), wants_grad(w),
+                         wants_grad(b));
+}
+
+}  // namespace
+
+void bind_blocks(py::module& m) {
+    m.def("fp8_blocks_quant", &fp8_blocks_quant);
+    m.def("fp8_blocks_dequant", &fp8_blocks_dequant);
+    m.def("fp8_blocks_matmul", &fp8_blocks_matmul);
+    m.def("linear_fp8", &linear_fp8);
+    m.def("linear_fp8_serve", &linear_fp8_serve);
+    m.def("layer_norm", &layer_norm);
+}

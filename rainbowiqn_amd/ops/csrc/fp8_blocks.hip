@@ -1,0 +1,715 @@
+// 8-bit block matrices for gfx950: e4m3 values with one power-of-two scale per
+// block of 128 columns and 1 or 128 rows, their products, and the backward
+// pass of a linear layer whose input is kept in that form.
+//
+// Layout of a matrix [R, C] with nb = ceil(C / 128):
+//   q     [R, 128 nb]            e4m3 bytes, zeros behind column C
+//   scale [R or ceil(R/128), S]  e8m0 bytes (e + 127), S = nb rounded up to 4
+// A value stands for q 2^e.  e = floor(log2(amax)) - 7 over the block's finite
+// values (0 for a block of zeros, at least -127), so |x| 2^-e < 256 stays
+// inside e4m3's 448 and every scale is a power of two: scaling is exact, and
+// the only rounding is the one to 4 significant bits (nearest, ties to even).
+// Values that are not finite become e4m3's NaN and leave the scale alone.
+//
+// Sums are fp32 throughout.  The matrix unit's 8-bit products keep less than
+// that: of 8 neighbouring products it drops what lies more than 16 bits under
+// the largest (seen with one product of 2^16 beside one of 1), which leaves
+// sums some 1e-5 of their size off.  e4m3 times a power of two is exact in
+// bf16, and bf16 products are summed in full: expanding the operands
+// (v_cvt_scalef32_pk_bf16_fp8, two values and their scale an instruction)
+// costs half the peak rate and nothing in precision.
+#include "common.h"
+#include "riqn_kernels.h"
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(2))) int i32x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+
+struct bf16_t { unsigned short v; };
+struct fp16_t { _Float16 v; };
+DEV float to_f(float x) { return x; }
+DEV float to_f(bf16_t x) { return bf16_to_f32(x.v); }
+DEV float to_f(fp16_t x) { return (float)x.v; }
+template <typename T> DEV T from_f(float x);
+template <> DEV float from_f<float>(float x) { return x; }
+template <> DEV bf16_t from_f<bf16_t>(float x) {
+    // the integer rounding of f32_to_bf16 would carry a NaN into infinity
+    return bf16_t{__builtin_bit_cast(unsigned short, (__bf16)x)};
+}
+template <> DEV fp16_t from_f<fp16_t>(float x) { return fp16_t{(_Float16)x}; }
+
+// relu and the truth value that its gradient goes by; NaN passes both
+DEV bool passes(float z) { return !(z <= 0.0f); }
+
+// 2^e for e in [-126, 127]
+DEV float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+DEV int block_exp(float amax) {
+    if (amax <= 0.0f) return 0;
+    return max((int)(__float_as_uint(amax) >> 23) - 134, -127);
+}
+
+// max over each group of 16 lanes, in every lane of it
+template <int N>
+DEV float ror16_max(float v) {
+    int o = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf,
+                                        0xf, false);
+    return fmaxf(v, __int_as_float(o));
+}
+DEV float max16(float v) {
+    v = ror16_max<8>(v);
+    v = ror16_max<4>(v);
+    v = ror16_max<2>(v);
+    return ror16_max<1>(v);
+}
+
+DEV float finite_abs(float x) {
+    const float a = fabsf(x);
+    return a < __builtin_inff() ? a : 0.0f;  // false for NaN too
+}
+
+// 8 scaled values -> 8 e4m3 bytes
+DEV i32x2 pack8(const float* v, float inv) {
+    i32x2 r;
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * inv,
+                                                v[4 * i + 1] * inv, 0, false);
+        r[i] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * inv,
+                                               v[4 * i + 3] * inv, w, true);
+    }
+    return r;
+}
+
+// 8 consecutive values of a row, zeros behind column C.  VEC: every 8th
+// element of every row is 16-byte aligned and C is a multiple of 8.
+template <typename T, bool VEC>
+DEV void load8(const T* p, int col, int C, float* v) {
+    if (VEC) {
+        if (col < C) {
+            struct alignas(16) Pack { T t[8]; };
+            const Pack x = *(const Pack*)(p + col);
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_f(x.t[i]);
+        } else {
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        }
+    } else {
+        #pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = col + i < C ? to_f(p[col + i]) : 0.0f;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Quantisation with a scale per 1 x 128 block.  16 lanes hold one block, 8
+// columns each; BPW blocks of a row per wave (1 for narrow matrices, so that
+// the wave's other lanes take further rows).  Bound by memory: reads the
+// input once, writes half (bf16) or a quarter (fp32) of it.
+//
+// MASK: values whose bit is clear are taken as zero (the gradient of a relu).
+// SUM: also adds up the columns, for the bias gradient: each workgroup writes
+// its partial sums in fp32 to part[blockIdx.y][C]; no atomics, so the result
+// does not depend on the order in which workgroups run.
+// ---------------------------------------------------------------------------
+template <typename T, bool VEC, int BPW, bool MASK, bool SUM>
+__global__ __launch_bounds__(256) void quant_rows_kernel(
+    const T* __restrict__ x, int64_t ldx, const uint8_t* __restrict__ mask,
+    uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
+    float* __restrict__ part, int R, int C, int nb, int S) {
+    constexpr int RPW = 4 / BPW;  // rows of a wave
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int grp = lane >> 4, l15 = lane & 15;
+    const int blk = blockIdx.x * BPW + (BPW == 4 ? grp : 0);
+    const int col = blk * 128 + l15 * 8;
+    const int step = 4 * RPW * gridDim.y;
+    float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (blk < nb) {
+        for (int r = (blockIdx.y * 4 + wave) * RPW + (BPW == 4 ? 0 : grp);
+             r < R; r += step) {
+            float v[8];
+            load8<T, VEC>(x + r * ldx, col, C, v);
+            if (MASK) {
+                const unsigned m = mask[(int64_t)r * (nb * 16) + blk * 16 + l15];
+                #pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = (m >> i) & 1 ? v[i] : 0.0f;
+            }
+            float am = 0.0f;
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                am = fmaxf(am, finite_abs(v[i]));
+                if (SUM) sum[i] += v[i];
+            }
+            const int e = block_exp(max16(am));
+            *(i32x2*)(q + (int64_t)r * (nb * 128) + col) = pack8(v, pow2i(-e));
+            if (l15 == 0) scale[(int64_t)r * S + blk] = (uint8_t)(e + 127);
+            // bytes between nb and S are read with the others as one dword
+            if (l15 == 0 && blk == nb - 1)
+                for (int i = nb; i < S; ++i) scale[(int64_t)r * S + i] = 0;
+        }
+    }
+    if (SUM) {
+        __shared__ float red[4][64][9];  // 9: lanes on different banks
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) red[wave][lane][i] = sum[i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < BPW * 128; c += 256) {
+            float t = 0.0f;
+            #pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                #pragma unroll
+                for (int g = 0; g < RPW; ++g)
+                    t += red[w][(BPW == 4 ? c >> 3 : g * 16 + (c >> 3))][c & 7];
+            }
+            const int cc = blockIdx.x * BPW * 128 + c;
+            if (cc < C) part[(int64_t)blockIdx.y * C + cc] = t;
+        }
+    }
+}
+
+// out[c] = sum over G rows of part[g][c]
+template <typename T>
+__global__ __launch_bounds__(256) void column_sum_kernel(
+    const float* __restrict__ part, T* __restrict__ out, int G, int C) {
+    __shared__ float red[8][32];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), g0 = threadIdx.x >> 5;
+    float t = 0.0f;
+    if (c < C)
+        for (int g = g0; g < G; g += 8) t += part[(int64_t)g * C + c];
+    red[g0][threadIdx.x & 31] = t;
+    __syncthreads();
+    if (g0 == 0 && c < C) {
+        #pragma unroll
+        for (int i = 1; i < 8; ++i) t += red[i][threadIdx.x];
+        out[c] = from_f<T>(t);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Quantisation with a scale per 128 x 128 block, for weights; qt/scale_t (may
+// be null) get the transposed matrix, whose blocks have the same scales.  One
+// workgroup per block: 64 values a thread stay in registers between the
+// maximum and the conversion; the transposed bytes go through LDS.
+// ---------------------------------------------------------------------------
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void quant_tiles_kernel(
+    const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
+    uint8_t* __restrict__ scale, uint8_t* __restrict__ qt,
+    uint8_t* __restrict__ scale_t, int R, int C, int nb, int S, int nbt,
+    int St) {
+    __shared__ float wmax[4];
+    __shared__ uint8_t tile[128][132];  // 132: columns fall on all banks
+    const int t = threadIdx.x, l15 = t & 15, rr = t >> 4;
+    const int bc = blockIdx.x, br = blockIdx.y;
+    const int col = bc * 128 + l15 * 8;
+    float v[8][8];
+    float am = 0.0f;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = br * 128 + i * 16 + rr;
+        if (r < R) {
+            load8<T, VEC>(x + r * ldx, col, C, v[i]);
+        } else {
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        }
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) am = fmaxf(am, finite_abs(v[i][j]));
+    }
+    #pragma unroll
+    for (int off = 32; off > 0; off >>= 1) am = fmaxf(am, __shfl_xor(am, off, 64));
+    if ((t & 63) == 0) wmax[t >> 6] = am;
+    __syncthreads();
+    am = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+    const int e = block_exp(am);
+    const float inv = pow2i(-e);
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = br * 128 + i * 16 + rr;
+        const i32x2 w = pack8(v[i], inv);
+        if (r < R) *(i32x2*)(q + (int64_t)r * (nb * 128) + col) = w;
+        if (qt) {
+            *(int*)&tile[i * 16 + rr][l15 * 8] = w[0];
+            *(int*)&tile[i * 16 + rr][l15 * 8 + 4] = w[1];
+        }
+    }
+    if (t == 0) {
+        scale[(int64_t)br * S + bc] = (uint8_t)(e + 127);
+        if (bc == nb - 1)
+            for (int i = nb; i < S; ++i) scale[(int64_t)br * S + i] = 0;
+        if (qt) {
+            scale_t[(int64_t)bc * St + br] = (uint8_t)(e + 127);
+            if (br == nbt - 1)
+                for (int i = nbt; i < St; ++i) scale_t[(int64_t)bc * St + i] = 0;
+        }
+    }
+    if (!qt) return;
+    __syncthreads();
+    // row c of the transposed block: 128 bytes, 8 per lane of 16
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int c = i * 16 + rr;
+        if (bc * 128 + c < C) {
+            uint32_t w[2] = {0, 0};
+            #pragma unroll
+            for (int j = 0; j < 8; ++j)
+                w[j >> 2] |= (uint32_t)tile[l15 * 8 + j][c] << (8 * (j & 3));
+            *(i32x2*)(qt + (int64_t)(bc * 128 + c) * (nbt * 128) + br * 128 +
+                      l15 * 8) = i32x2{(int)w[0], (int)w[1]};
+        }
+    }
+}
+
+// 8-bit blocks -> T; 8 columns a thread.  q 2^e is exact in fp32, and in bf16
+// wherever it is a normal number.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void dequant_kernel(
+    const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale,
+    T* __restrict__ out, int R, int C, int nb, int S, int shift) {
+    const int per = (C + 7) >> 3;  // groups of 8 columns in a row
+    for (int64_t i = threadIdx.x + (int64_t)blockIdx.x * 256;
+         i < (int64_t)R * per; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per;
+        const int col = (int)(i - r * per) * 8;
+        const i32x2 w = *(const i32x2*)(q + r * (nb * 128) + col);
+        const int e = (int)scale[(r >> shift) * S + (col >> 7)] - 127;
+        // 2^-127 is no normal number: two factors, each a power of two
+        const float s0 = pow2i(e < 0 ? e + 1 : e), s1 = e < 0 ? 0.5f : 1.0f;
+        struct alignas(16) Pack { T t[8]; } p;
+        #pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false);
+            auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
+            p.t[4 * j] = from_f<T>(lo[0] * s0 * s1);
+            p.t[4 * j + 1] = from_f<T>(lo[1] * s0 * s1);
+            p.t[4 * j + 2] = from_f<T>(hi[0] * s0 * s1);
+            p.t[4 * j + 3] = from_f<T>(hi[1] * s0 * s1);
+        }
+        T* o = out + r * C + col;
+        if (VEC) {
+            *(Pack*)o = p;
+        } else {
+            #pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (col + j < C) o[j] = p.t[j];
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// C[m][n] = sum_k A[m][k] B[n][k] (+ bias[n], relu).  The MFMA's row operand
+// is B, so a lane's 4 results are 4 neighbours of one row of C.
+// ---------------------------------------------------------------------------
+struct Gemm {
+    const uint8_t *a, *as, *b, *bs;  // [M, 128 nb], [M >> ash, S] and so on
+    const void* bias;                // [N] of bias_t, or null
+    void* c;                         // [M, N]
+    uint8_t* mask;                   // [M, 16 ceil(N / 128)] bits, or null
+    int M, N, nb, S, ash, bsh, bias_t, relu;
+};
+
+DEV float bias_at(const Gemm& g, int n) {
+    if (!g.bias) return 0.0f;
+    return g.bias_t == 0   ? ((const float*)g.bias)[n]
+           : g.bias_t == 1 ? to_f(((const bf16_t*)g.bias)[n])
+                           : to_f(((const fp16_t*)g.bias)[n]);
+}
+
+// 8 e4m3 values and a scale byte -> bf16.  The conversion takes the exponent
+// field of its fp32 scale alone, so a byte of 0 stands for 2^-127.
+DEV bf16x8 expand8(int w0, int w1, int sbyte) {
+    const float s = __uint_as_float((uint32_t)sbyte << 23);
+    union { bf16x2 h[4]; bf16x8 v; } u;
+    u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, false);
+    u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, true);
+    u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, false);
+    u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, true);
+    return u.v;
+}
+
+// Few rows or small results: a workgroup of 8 waves computes a tile of
+// 16 MI x 16 NI, each wave a share of the 128-column blocks (kb = wave,
+// wave + 8, ...), with operands straight from memory into registers: no
+// staging, so a wave has all its loads in flight at once.  The 8 partial
+// tiles are added in LDS in a fixed order.  Bound by latency, so the products
+// are the exact bf16 ones.
+template <int MI, int NI, typename T>
+__global__ __launch_bounds__(512) void gemm_direct_kernel(Gemm g) {
+    constexpr int TM = 16 * MI, TN = 16 * NI;
+    __shared__ float red[8][TM][TN + 4];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int l15 = lane & 15, l4 = lane >> 4;
+    const int nt = (g.N + TN - 1) / TN;
+    const int m0 = (blockIdx.x / nt) * TM, n0 = (blockIdx.x % nt) * TN;
+    const int64_t ld = (int64_t)g.nb * 128;
+    const uint8_t *pa[MI], *sa[MI], *pb[NI], *sb[NI];
+    #pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        const int64_t r = min(m0 + i * 16 + l15, g.M - 1);
+        pa[i] = g.a + r * ld + l4 * 16;
+        sa[i] = g.as + (r >> g.ash) * g.S;
+    }
+    #pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int64_t r = min(n0 + i * 16 + l15, g.N - 1);
+        pb[i] = g.b + r * ld + l4 * 16;
+        sb[i] = g.bs + (r >> g.bsh) * g.S;
+    }
+    f32x4 acc[MI][NI];
+    #pragma unroll
+    for (int i = 0; i < MI; ++i)
+        #pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    #pragma unroll 2
+    for (int kb = wave; kb < g.nb; kb += 8) {
+        i32x4 fa[MI][2], fb[NI][2];
+        int ea[MI], eb[NI];
+        #pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            fa[i][0] = *(const i32x4*)(pa[i] + kb * 128);
+            fa[i][1] = *(const i32x4*)(pa[i] + kb * 128 + 64);
+            ea[i] = sa[i][kb];
+        }
+        #pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            fb[i][0] = *(const i32x4*)(pb[i] + kb * 128);
+            fb[i][1] = *(const i32x4*)(pb[i] + kb * 128 + 64);
+            eb[i] = sb[i][kb];
+        }
+        // the order of the 128 products is free, as both operands have it
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            #pragma unroll
+            for (int u = 0; u < 4; u += 2) {
+                bf16x8 xb[NI];
+                #pragma unroll
+                for (int j = 0; j < NI; ++j)
+                    xb[j] = expand8(fb[j][h][u], fb[j][h][u + 1], eb[j]);
+                #pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    const bf16x8 xa =
+                        expand8(fa[i][h][u], fa[i][h][u + 1], ea[i]);
+                    #pragma unroll
+                    for (int j = 0; j < NI; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            xb[j], xa, acc[i][j], 0, 0, 0);
+                }
+            }
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < MI; ++i)
+        #pragma unroll
+        for (int j = 0; j < NI; ++j)
+            *(f32x4*)&red[wave][i * 16 + l15][j * 16 + l4 * 4] = acc[i][j];
+    __syncthreads();
+    constexpr int QUADS = TM * TN / 4;
+    if (t >= QUADS) return;
+    const int mm = t / (TN / 4), nn = (t % (TN / 4)) * 4;
+    f32x4 z = *(const f32x4*)&red[0][mm][nn];
+    #pragma unroll
+    for (int w = 1; w < 8; ++w) z += *(const f32x4*)&red[w][mm][nn];
+    const int m = m0 + mm, n = n0 + nn;
+    unsigned bits = 0;
+    struct alignas(4 * sizeof(T)) Pack { T t[4]; } p;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float y = z[j] + (n + j < g.N ? bias_at(g, n + j) : 0.0f);
+        const bool on = passes(y);
+        bits |= (unsigned)(on && n + j < g.N) << j;
+        if (g.relu && !on) y = 0.0f;
+        p.t[j] = from_f<T>(y);
+    }
+    if (g.mask) {
+        // four neighbours make 16 columns; quads of a row are 4-aligned
+        bits <<= 4 * (t & 3);
+        bits |= __shfl_xor(bits, 1, 64);
+        bits |= __shfl_xor(bits, 2, 64);
+        if ((t & 3) == 0 && m < g.M)
+            *(uint16_t*)(g.mask + (int64_t)m * (((g.N + 127) >> 7) * 16) +
+                         (n >> 3)) = (uint16_t)bits;
+    }
+    if (m >= g.M) return;
+    T* out = (T*)g.c + (int64_t)m * g.N + n;
+    if ((g.N & 3) == 0) {
+        if (n < g.N) *(Pack*)out = p;
+    } else {
+        #pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (n + j < g.N) out[j] = p.t[j];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// dW[n][k] = sum_m G[m][n] X[m][k]: both operands have a scale per row m, the
+// summed index, so tiles are expanded to bf16 on their way into LDS; nothing
+// is rounded before the fp32 sums.  LDS keeps rows of m; ds_read_b64_tr_b16 hands each lane 4
+// rows of one column, the operand layout of a product that sums over rows.
+//
+// A tile is 128 x 128, one block of each operand, 64 rows a step, 4 waves of
+// 64 x 64.  The 256-byte LDS rows are stored in 32-byte pieces at piece ^
+// (row & 7), so that the 16 rows of a transposed read fall on all banks.
+// blockIdx.y takes a share of the rows; with more than one share each writes
+// fp32 partials [share][N][K], added in a fixed order by add_shares_kernel.
+// ---------------------------------------------------------------------------
+struct Wgrad {
+    const uint8_t *g, *gs, *x, *xs;  // [M, 128 nbn], [M, Sn], [M, 128 nbk], ...
+    void* dw;                        // [N, K] of T, or fp32 [shares][N][K]
+    int M, N, K, nbn, Sn, nbk, Sk, rows;  // rows of a share: multiple of 64
+};
+
+// the 16 rows m = l4 * 4 ... of 16 columns from c: bf16 [64][128] swizzled
+DEV bf16x8 tr_frag(const uint16_t* tile, int m, int c, int lane) {
+    const int l15 = lane & 15, l4 = lane >> 4;
+    bf16x8 f;
+    #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = m + h * 16 + l4 * 4 + (l15 >> 2);
+        const int piece = (c >> 4) ^ (row & 7);
+        auto* p = (__attribute__((address_space(3))) s16x4*)(
+            tile + row * 128 + piece * 16 + (l15 & 3) * 4);
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
+        const bf16x4 b = __builtin_bit_cast(bf16x4, v);
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) f[h * 4 + j] = b[j];
+    }
+    return f;
+}
+
+DEV void expand_store(uint16_t* tile, int row, int piece, i32x4 w, int sbyte) {
+    // 16 values = one 32-byte piece of the row
+    i32x4* p = (i32x4*)(tile + row * 128 + (piece ^ (row & 7)) * 16);
+    p[0] = __builtin_bit_cast(i32x4, expand8(w[0], w[1], sbyte));
+    p[1] = __builtin_bit_cast(i32x4, expand8(w[2], w[3], sbyte));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void wgrad_kernel(Wgrad w) {
+    __shared__ __align__(16) uint16_t gt[64 * 128], xt[64 * 128];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int l15 = lane & 15, l4 = lane >> 4;
+    const int bn = blockIdx.x / w.nbk, bk = blockIdx.x % w.nbk;
+    const int wn = (wave >> 1) * 64, wk = (wave & 1) * 64;
+    const int64_t ldg = (int64_t)w.nbn * 128, ldx = (int64_t)w.nbk * 128;
+    const int lo = blockIdx.y * w.rows, hi = min(lo + w.rows, w.M);
+    f32x4 acc[4][4];
+    #pragma unroll
+    for (int i = 0; i < 4; ++i)
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    for (int m0 = lo; m0 < hi; m0 += 64) {
+        // 64 rows x 8 pieces of 16 bytes: 2 per thread and operand
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = i * 32 + (t >> 3), piece = t & 7;
+            const int64_t m = m0 + row;
+            i32x4 gv = {0, 0, 0, 0}, xv = {0, 0, 0, 0};
+            int ge = 127, xe = 127;
+            if (m < hi) {
+                gv = *(const i32x4*)(w.g + m * ldg + bn * 128 + piece * 16);
+                xv = *(const i32x4*)(w.x + m * ldx + bk * 128 + piece * 16);
+                ge = w.gs[m * w.Sn + bn];
+                xe = w.xs[m * w.Sk + bk];
+            }
+            expand_store(gt, row, piece, gv, ge);
+            expand_store(xt, row, piece, xv, xe);
+        }
+        __syncthreads();
+        #pragma unroll
+        for (int ms = 0; ms < 64; ms += 32) {
+            bf16x8 fg[4], fx[4];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                fg[i] = tr_frag(gt, ms, wn + i * 16, lane);
+                fx[i] = tr_frag(xt, ms, wk + i * 16, lane);
+            }
+            // rows of the result are k, so a lane holds 4 neighbours of a row
+            #pragma unroll
+            for (int i = 0; i < 4; ++i)
+                #pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        fx[j], fg[i], acc[i][j], 0, 0, 0);
+        }
+        __syncthreads();
+    }
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = bn * 128 + wn + i * 16 + l15;
+        if (n >= w.N) continue;
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = bk * 128 + wk + j * 16 + l4 * 4;
+            T* out = (T*)w.dw + ((int64_t)blockIdx.y * w.N + n) * w.K + k;
+            struct alignas(4 * sizeof(T)) Pack { T t[4]; } p;
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) p.t[e] = from_f<T>(acc[i][j][e]);
+            if ((w.K & 3) == 0) {
+                if (k < w.K) *(Pack*)out = p;
+            } else {
+                #pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (k + e < w.K) out[e] = p.t[e];
+            }
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void add_shares_kernel(
+    const float* __restrict__ part, T* __restrict__ out, int shares,
+    int64_t n) {
+    for (int64_t i = threadIdx.x + (int64_t)blockIdx.x * 256; i < n;
+         i += (int64_t)gridDim.x * 256) {
+        float t = part[i];
+        for (int s = 1; s < shares; ++s) t += part[s * n + i];
+        out[i] = from_f<T>(t);
+    }
+}
+
+#define RIQN_TYPE(code, T, ...)                     \
+    switch (code) {                                 \
+        case 0: { using T = float; __VA_ARGS__; } break;   \
+        case 1: { using T = bf16_t; __VA_ARGS__; } break;  \
+        default: { using T = fp16_t; __VA_ARGS__; } break; \
+    }
+
+bool vec8(const void* p, int64_t ld, int C, int type) {
+    const int size = type == 0 ? 4 : 2;
+    return ((uintptr_t)p & 15) == 0 && (ld * size & 15) == 0 && (C & 7) == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int riqn_fp8_quant_rows(const void* x, int type, int64_t ldx,
+                        const uint8_t* mask, uint8_t* q, uint8_t* scale,
+                        float* part, int groups, int R, int C, void* stream) {
+    const int nb = (C + 127) >> 7, S = (nb + 3) & ~3;
+    const bool wide = nb >= 4, vec = vec8(x, ldx, C, type);
+    dim3 grid(wide ? (nb + 3) / 4 : nb, groups);
+    hipStream_t st = (hipStream_t)stream;
+#define RIQN_Q4(V, B, MK, SM)                                              \
+    hipLaunchKernelGGL((quant_rows_kernel<T, V, B, MK, SM>), grid,         \
+                       dim3(256), 0, st, (const T*)x, ldx, mask, q, scale, \
+                       part, R, C, nb, S)
+#define RIQN_Q3(V, B)                     \
+    if (mask && part) RIQN_Q4(V, B, true, true);         \
+    else if (mask) RIQN_Q4(V, B, true, false);           \
+    else if (part) RIQN_Q4(V, B, false, true);           \
+    else RIQN_Q4(V, B, false, false)
+    RIQN_TYPE(type, T, {
+        if (vec && wide) { RIQN_Q3(true, 4); }
+        else if (vec) { RIQN_Q3(true, 1); }
+        else if (wide) { RIQN_Q3(false, 4); }
+        else { RIQN_Q3(false, 1); }
+    })
+    return (int)hipGetLastError();
+}
+
+int riqn_column_sum(const float* part, void* out, int type, int G, int C,
+                    void* stream) {
+    RIQN_TYPE(type, T, hipLaunchKernelGGL(
+        column_sum_kernel<T>, dim3((C + 31) / 32), dim3(256), 0,
+        (hipStream_t)stream, part, (T*)out, G, C))
+    return (int)hipGetLastError();
+}
+
+int riqn_fp8_quant_tiles(const void* x, int type, int64_t ldx, uint8_t* q,
+                         uint8_t* scale, uint8_t* qt, uint8_t* scale_t, int R,
+                         int C, void* stream) {
+    const int nb = (C + 127) >> 7, nbt = (R + 127) >> 7;
+    const bool vec = vec8(x, ldx, C, type);
+    RIQN_TYPE(type, T, {
+        if (vec)
+            hipLaunchKernelGGL((quant_tiles_kernel<T, true>), dim3(nb, nbt),
+                               dim3(256), 0, (hipStream_t)stream, (const T*)x,
+                               ldx, q, scale, qt, scale_t, R, C, nb,
+                               (nb + 3) & ~3, nbt, (nbt + 3) & ~3);
+        else
+            hipLaunchKernelGGL((quant_tiles_kernel<T, false>), dim3(nb, nbt),
+                               dim3(256), 0, (hipStream_t)stream, (const T*)x,
+                               ldx, q, scale, qt, scale_t, R, C, nb,
+                               (nb + 3) & ~3, nbt, (nbt + 3) & ~3);
+    })
+    return (int)hipGetLastError();
+}
+
+int riqn_fp8_dequant(const uint8_t* q, const uint8_t* scale, void* out,
+                     int type, int R, int C, int shift, void* stream) {
+    const int nb = (C + 127) >> 7, S = (nb + 3) & ~3;
+    const int64_t n = (int64_t)R * ((C + 7) >> 3);
+    const uint32_t blocks = (uint32_t)min((n + 255) / 256, (int64_t)1 << 20);
+    const bool vec = vec8(out, C, C, type);
+    RIQN_TYPE(type, T, {
+        if (vec)
+            hipLaunchKernelGGL((dequant_kernel<T, true>), dim3(blocks),
+                               dim3(256), 0, (hipStream_t)stream, q, scale,
+                               (T*)out, R, C, nb, S, shift);
+        else
+            hipLaunchKernelGGL((dequant_kernel<T, false>), dim3(blocks),
+                               dim3(256), 0, (hipStream_t)stream, q, scale,
+                               (T*)out, R, C, nb, S, shift);
+    })
+    return (int)hipGetLastError();
+}
+
+int riqn_fp8_gemm(const uint8_t* a, const uint8_t* as, int a_block_rows,
+                  const uint8_t* b, const uint8_t* bs, int b_block_rows,
+                  const void* bias, int bias_type, int relu, void* c,
+                  int c_type, uint8_t* mask, int M, int N, int K,
+                  void* stream) {
+    const int nb = (K + 127) >> 7;
+    Gemm g{a, as, b, bs, bias, c, mask, M, N, nb, (nb + 3) & ~3,
+           a_block_rows == 128 ? 7 : 0, b_block_rows == 128 ? 7 : 0, bias_type,
+           relu};
+    hipStream_t st = (hipStream_t)stream;
+    RIQN_TYPE(c_type, T, {
+        if (M <= 16) {
+            const uint32_t tiles = (N + 15) / 16;
+            hipLaunchKernelGGL((gemm_direct_kernel<1, 1, T>), dim3(tiles),
+                               dim3(512), 0, st, g);
+        } else {
+            const int64_t tiles =
+                (int64_t)((M + 31) / 32) * ((N + 31) / 32);
+            hipLaunchKernelGGL((gemm_direct_kernel<2, 2, T>),
+                               dim3((uint32_t)tiles), dim3(512), 0, st, g);
+        }
+    })
+    return (int)hipGetLastError();
+}
+
+int riqn_fp8_wgrad(const uint8_t* g, const uint8_t* gs, const uint8_t* x,
+                   const uint8_t* xs, void* dw, int type, float* part,
+                   int shares, int M, int N, int K, void* stream) {
+    const int nbn = (N + 127) >> 7, nbk = (K + 127) >> 7;
+    const int rows = ((M + shares - 1) / shares + 63) & ~63;
+    Wgrad w{g, gs, x, xs, shares > 1 ? (void*)part : dw, M, N, K, nbn,
+            (nbn + 3) & ~3, nbk, (nbk + 3) & ~3, rows};
+    hipStream_t st = (hipStream_t)stream;
+    dim3 grid(nbn * nbk, shares);
+    RIQN_TYPE(shares > 1 ? 0 : type, T, hipLaunchKernelGGL(
+        wgrad_kernel<T>, grid, dim3(256), 0, st, w))
+    if (shares > 1) {
+        const int64_t n = (int64_t)N * K;
+        RIQN_TYPE(type, T, hipLaunchKernelGGL(
+            add_shares_kernel<T>,
+            dim3((uint32_t)min((n + 255) / 256, (int64_t)4096)), dim3(256), 0,
+            st, part, (T*)dw, shares, n))
+    }
+    return (int)hipGetLastError();
+}
+
+}  // extern "C"

@@ -154,6 +154,36 @@ void riqn_heads_gemm_fp8(const void* hq, const void* hsc, const void* wq,
                          const void* wsc, const void* bcat, void* out, int R,
                          int variant, void* stream);
 
+// ---- 8-bit block matrices (fp8_blocks.hip) ----------------------------------
+// These return a hipError_t as int.  Types: 0 fp32, 1 bf16, 2 fp16.
+int riqn_fp8_quant_rows(const void* x, int type, int64_t ldx,
+                        const uint8_t* mask, uint8_t* q, uint8_t* scale,
+                        float* part, int groups, int R, int C, void* stream);
+int riqn_column_sum(const float* part, void* out, int type, int G, int C,
+                    void* stream);
+int riqn_fp8_quant_tiles(const void* x, int type, int64_t ldx, uint8_t* q,
+                         uint8_t* scale, uint8_t* qt, uint8_t* scale_t, int R,
+                         int C, void* stream);
+int riqn_fp8_dequant(const uint8_t* q, const uint8_t* scale, void* out,
+                     int type, int R, int C, int shift, void* stream);
+int riqn_fp8_gemm(const uint8_t* a, const uint8_t* as, int a_block_rows,
+                  const uint8_t* b, const uint8_t* bs, int b_block_rows,
+                  const void* bias, int bias_type, int relu, void* c,
+                  int c_type, uint8_t* mask, int M, int N, int K,
+                  void* stream);
+int riqn_fp8_wgrad(const uint8_t* g, const uint8_t* gs, const uint8_t* x,
+                   const uint8_t* xs, void* dw, int type, float* part,
+                   int shares, int M, int N, int K, void* stream);
+
+// ---- layer norm (norm.hip) ---------------------------------------------------
+int riqn_norm_fwd(const void* x, int type, int64_t ldx, const void* w,
+                  const void* b, int wtype, void* y, float* mean, float* rstd,
+                  int R, int C, float eps, void* stream);
+int riqn_norm_bwd(const void* dy, const void* x, int type, int64_t lddy,
+                  int64_t ldx, const void* w, int wtype, const float* mean,
+                  const float* rstd, void* dx, void* dw, void* db, float* part,
+                  int groups, int R, int C, void* stream);
+
 // batched 4-layer NoisyLinear regeneration (rng.hip)
 struct NoisyDesc {
     const void *w_mu, *w_sigma, *b_mu, *b_sigma;

@@ -61,3 +61,49 @@ def preprocess_frames(frames_u8: torch.Tensor, dtype=torch.float32) -> torch.Ten
 def argmax_mean_quantiles(z: torch.Tensor) -> torch.Tensor:
     """z: [B, K, A] -> greedy action per sample  (kernel K9)."""
     return z.mean(dim=1).argmax(dim=1)
+
+
+# -- 8-bit block matrices and layer norm -------------------------------------
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last axis, computed in fp32 and rounded once."""
+    xf = x.float()
+    c = xf - xf.mean(-1, keepdim=True)
+    y = c * torch.rsqrt((c * c).mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        y = y * weight.float()
+    if bias is not None:
+        y = y + bias.float()
+    return y.to(x.dtype)
+
+
+def _pow2(e: torch.Tensor) -> torch.Tensor:
+    """2^e in fp32 from the exponent field of a double (exact; e >= -127)."""
+    return ((e.to(torch.int64) + 1023) << 52).view(torch.float64).float()
+
+
+def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1):
+    """x [R, C] -> (q, scale) of Fp8Blocks (ops/functional.py).
+
+    Per block of `block_rows` x 128: e = floor(log2(amax)) - 7 over its finite
+    values, at least -127, 0 for a block of zeros; q = e4m3(x 2^-e), ties to
+    even; values that are not finite become NaN."""
+    r, c = x.shape
+    t = torch.nn.functional.pad(x.float(), (0, -c % 128, 0, -r % block_rows))
+    t = t.reshape(-(-r // block_rows), block_rows, -(-c // 128), 128)
+    a = torch.where(torch.isfinite(t), t.abs(), torch.zeros_like(t))
+    amax = a.amax(dim=(1, 3), keepdim=True)
+    e = torch.clamp((amax.view(torch.int32) >> 23) - 134, min=-127)
+    e = torch.where(amax > 0, e, torch.zeros_like(e))
+    v = torch.where(torch.isfinite(t), t, torch.full_like(t, float("nan")))
+    q = (v * _pow2(-e)).to(torch.float8_e4m3fn).view(torch.uint8)
+    q = q.reshape(q.shape[0] * block_rows, q.shape[2] * 128)[:r].contiguous()
+    s = (e.reshape(e.shape[0], e.shape[2]) + 127).to(torch.uint8)
+    return q, torch.nn.functional.pad(s, (0, -s.shape[1] % 4)).contiguous()
+
+
+def dequantize_fp8_blocks(q, scale, cols: int, block_rows: int,
+                          dtype=torch.float32) -> torch.Tensor:
+    e = scale[:, :q.shape[1] // 128].to(torch.int32) - 127
+    e = e.repeat_interleave(block_rows, 0)[:q.shape[0]].repeat_interleave(128, 1)
+    v = q.view(torch.float8_e4m3fn).float() * _pow2(e)
+    return v[:, :cols].to(dtype).contiguous()

@@ -20,6 +20,7 @@ ext = CUDAExtension(
     name="rainbowiqn_amd.ops._rainbowiqn_hip",
     sources=[
         os.path.join(CSRC, "bindings.cpp"),
+        os.path.join(CSRC, "bindings_blocks.cpp"),
         os.path.join(CSRC, "replay.hip"),
         os.path.join(CSRC, "loss.hip"),
         os.path.join(CSRC, "adam.hip"),
@@ -28,6 +29,8 @@ ext = CUDAExtension(
         os.path.join(CSRC, "model_fwd.hip"),
         os.path.join(CSRC, "model_bwd.hip"),
         os.path.join(CSRC, "model_fp8.hip"),
+        os.path.join(CSRC, "fp8_blocks.hip"),
+        os.path.join(CSRC, "norm.hip"),
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],

@@ -1,0 +1,500 @@
+"""8-bit block matrices: quantisation, products, the linear layer that keeps its
+input in 8 bits (ops/functional.py), against plain 64-bit forms.
+
+Tolerances, all fixed beforehand.  Quantisation is exact scaling and one
+rounding, so bytes are compared for equality.  A sum of n products in fp32, in
+any order, is off by at most n 2^-24 times the sum of their magnitudes (Higham,
+Accuracy and Stability, eq. 3.5, with n 2^-24 << 1); 8-bit products that the
+matrix unit sums in groups of 8 lose bits 16 under the largest of a group, at
+most 8 x 2^-16 of it, which 2^-13 times the sum of magnitudes covers.  The
+result's own rounding adds half a step, eps / 2 of its value."""
+
+import pytest
+import torch
+
+from rainbowiqn_amd.ops import functional as F
+from rainbowiqn_amd.ops import torch_ref
+from rainbowiqn_amd.ops.functional import Fp8Blocks
+
+gpu = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def e4m3_grid(v):
+    """v (fp64, |v| < 448) to 4 significant bits, steps of 2^-9 below 2^-6."""
+    _, e = torch.frexp(v)
+    step = torch.clamp(e - 4, min=-9).double()
+    return torch.round(v / 2 ** step) * 2 ** step
+
+
+def held(x, block_rows=1):
+    """What 8-bit blocks make of x, in 64 bits on the CPU, from the definition."""
+    x = x.detach().double().cpu()
+    r, c = x.shape
+    t = torch.nn.functional.pad(x, (0, -c % 128, 0, -r % block_rows))
+    t = t.reshape(-(-r // block_rows), block_rows, -(-c // 128), 128)
+    top = t.abs().amax(dim=(1, 3), keepdim=True)
+    e = (torch.frexp(top)[1] - 8).clamp(min=-127)
+    scale = 2.0 ** torch.where(top > 0, e, torch.zeros_like(e)).double()
+    t = e4m3_grid(t / scale) * scale
+    return t.reshape(t.shape[0] * block_rows, t.shape[2] * 128)[:r, :c]
+
+
+def tol(n, magnitude, out, dtype):
+    """The bound of the module's docstring, elementwise; results in fp32 come
+    from exact products."""
+    unit = n * 2.0 ** -24 + (0 if dtype == torch.float32 else 2.0 ** -13)
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    return unit * magnitude + torch.finfo(dtype).eps / 2 * out.abs() + tiny
+
+
+def near(got, want, bound):
+    most = torch.finfo(got.dtype).max
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape
+    off = (got - want).abs() - bound
+    # rounding takes what is past the type's range to infinity: the last finite
+    # number plus half a step, 1 + 2^-12 of it in fp16 and more in the others,
+    # which `bound` covers with its eps / 2 of the value
+    past = (want.abs() + bound >= most) & (got == want.sign() * float("inf"))
+    off = torch.where(past, torch.zeros_like(off), off)
+    assert bool((off <= 0).all()), float(off.max())
+
+
+def matrix(r, c, seed, dtype=torch.float32, device="cpu"):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(r, c, generator=g) * torch.exp(2 * torch.randn(r, 1, generator=g))
+    return x.to(dtype).to(device)
+
+
+# -- CPU: semantics and refusals -----------------------------------------------
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 127), (130, 129), (5, 640)])
+def test_ref_quantisation_is_the_definition(shape, block_rows):
+    x = matrix(*shape, seed=1)
+    b = F.quantize_fp8_blocks(x, block_rows)
+    assert b.shape == shape
+    assert torch.equal(F.dequantize_fp8_blocks(b).double(), held(x, block_rows))
+
+
+def test_ref_layout():
+    b = F.quantize_fp8_blocks(torch.ones(3, 130))
+    assert b.q.shape == (3, 256) and b.scale.shape == (3, 4)
+    assert int(b.q[:, 130:].sum()) == 0 and int(b.scale[:, 2:].sum()) == 0
+    # 1 = 128 * 2^-7
+    assert (b.scale[:, :2] == 127 - 7).all()
+    w = F.quantize_fp8_blocks(torch.ones(130, 3), 128)
+    assert w.q.shape == (130, 128) and w.scale.shape == (2, 4)
+
+
+@pytest.mark.parametrize("relu", [False, True])
+def test_cpu_linear_gradients_follow_the_formula(relu):
+    x, w = matrix(9, 200, 1).requires_grad_(), matrix(33, 200, 2).requires_grad_()
+    b = torch.randn(33, generator=torch.Generator().manual_seed(3)).requires_grad_()
+    dy = matrix(9, 33, 4)
+    y = F.linear_fp8_blocks(x, w, b, relu)
+    y.backward(dy)
+    check_linear(x, w, b, dy, y, x.grad, w.grad, b.grad, relu)
+
+
+def check_linear(x, w, b, dy, y, dx, dw, db, relu):
+    xh, wh, dt = held(x), held(w, 128), x.dtype
+    k, n, m = x.shape[1], w.shape[0], x.shape[0]
+    z = xh @ wh.t() + (b.detach().double().cpu() if b is not None else 0)
+    size = xh.abs() @ wh.abs().t() + (b.detach().double().cpu().abs() if b is not None else 0)
+    near(y, z.clamp(min=0) if relu else z, tol(k + 1, size, z, dt))
+    dz = dy.detach().double().cpu()
+    if relu:  # a sum next to zero may fall on either side: as y has it
+        dz = dz * (y.detach().double().cpu() > 0)
+    g = held(dz)
+    if dx is not None:
+        want = g @ wh
+        near(dx, want, tol(n, g.abs() @ wh.abs(), want, dx.dtype))
+    if dw is not None:
+        want = g.t() @ xh
+        # always from exact products: the bound of fp32 sums
+        near(dw, want, tol(m, g.abs().t() @ xh.abs(), want, torch.float32)
+             + torch.finfo(dw.dtype).eps / 2 * want.abs()
+             + torch.finfo(dw.dtype).smallest_normal)
+    if db is not None:
+        want = dz.sum(0)
+        near(db, want, tol(m, dz.abs().sum(0), want, torch.float32)
+             + torch.finfo(db.dtype).eps / 2 * want.abs())
+
+
+def refusals(device):
+    x = torch.randn(4, 200, device=device)
+    w = torch.randn(8, 200, device=device)
+    a, b = F.quantize_fp8_blocks(x), F.quantize_fp8_blocks(w, 128)
+    bad = RuntimeError
+    calls = [
+        lambda: F.quantize_fp8_blocks(x, 64),
+        lambda: F.quantize_fp8_blocks(x[0]),
+        lambda: F.quantize_fp8_blocks(x.long()),
+        lambda: F.quantize_fp8_blocks(x[:, :0]),
+        lambda: F.matmul_fp8_blocks(a, F.quantize_fp8_blocks(w[:, :100], 128)),
+        lambda: F.matmul_fp8_blocks(a, b, bias=torch.zeros(7, device=device)),
+        lambda: F.matmul_fp8_blocks(a._replace(q=a.q[:, :128]), b),
+        lambda: F.matmul_fp8_blocks(a._replace(scale=a.scale[:3]), b),
+        lambda: F.matmul_fp8_blocks(a._replace(scale=a.scale[:, :2]), b),
+        lambda: F.matmul_fp8_blocks(a._replace(block_rows=128), b),
+        lambda: F.matmul_fp8_blocks(a._replace(block_rows=2), b),
+        lambda: F.matmul_fp8_blocks(a._replace(q=a.q.to(torch.int8)), b),
+        lambda: F.dequantize_fp8_blocks(a._replace(cols=300)),
+        lambda: F.dequantize_fp8_blocks(a._replace(cols=0)),
+        lambda: F.linear_fp8_blocks(x, w[:, :100]),
+        lambda: F.linear_fp8_blocks(x, w, torch.zeros(9, device=device)),
+        lambda: F.linear_fp8_blocks(x, w[:0]),
+        lambda: F.linear_fp8_blocks(x[:, :0], w[:, :0]),
+        lambda: F.linear_fp8_blocks(x.long(), w),
+        lambda: F.linear_fp8_blocks(x[:, :100], b),
+        lambda: F.linear_fp8_blocks(x.clone().requires_grad_(), b),
+        lambda: F.linear_fp8_blocks(x, w, torch.zeros(1, 8, device=device)),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(bad):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    # a second derivative raises instead of counting as zero
+    x.requires_grad_()
+    y = F.linear_fp8_blocks(x, w)
+    (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(bad):
+        g.sum().backward()
+
+
+def test_refusals_cpu():
+    refusals("cpu")
+
+
+@gpu
+def test_refusals_gpu():
+    refusals("cuda")
+    x, w = torch.randn(4, 200, device="cuda"), torch.randn(8, 200)
+    a, b = F.quantize_fp8_blocks(x), F.quantize_fp8_blocks(w, 128)
+    for call in (lambda: F.linear_fp8_blocks(x, w),
+                 lambda: F.matmul_fp8_blocks(a, b),
+                 lambda: F.linear_fp8_blocks(x, b),
+                 lambda: F.linear_fp8_blocks(x, w.cuda(), torch.zeros(8)),
+                 lambda: F.matmul_fp8_blocks(a._replace(q=a.q.t().contiguous().t()), a),
+                 lambda: F.dequantize_fp8_blocks(a, torch.int32)):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def test_no_rows_cpu():
+    no_rows("cpu")
+
+
+@gpu
+def test_no_rows_gpu():
+    no_rows("cuda")
+
+
+def no_rows(device):
+    x = torch.zeros(0, 200, device=device, requires_grad=True)
+    w = torch.randn(8, 200, device=device, requires_grad=True)
+    b = torch.randn(8, device=device, requires_grad=True)
+    y = F.linear_fp8_blocks(x, w, b, relu=True)
+    assert y.shape == (0, 8)
+    y.sum().backward()
+    assert x.grad.shape == (0, 200)
+    assert not w.grad.any() and not b.grad.any() and w.grad.shape == w.shape
+    q = F.quantize_fp8_blocks(x)
+    assert q.shape == (0, 200) and F.dequantize_fp8_blocks(q).shape == (0, 200)
+    assert F.matmul_fp8_blocks(q, F.quantize_fp8_blocks(w, 128)).shape == (0, 8)
+    with torch.no_grad():
+        assert F.linear_fp8_blocks(x, F.quantize_fp8_blocks(w, 128)).shape == (0, 8)
+
+
+# -- GPU: quantisation ----------------------------------------------------------
+def equal_blocks(got, x, block_rows):
+    q, s = torch_ref.quantize_fp8_blocks(x.detach().cpu(), block_rows)
+    assert torch.equal(got.scale.cpu(), s)
+    # a NaN's sign is not part of its value
+    nan = (q & 0x7F) == 0x7F
+    assert torch.equal((got.q.cpu() & 0x7F) == 0x7F, nan)
+    assert torch.equal(got.q.cpu()[~nan], q[~nan])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("shape", [
+    (1, 1), (1, 128), (2, 127), (3, 129), (17, 511), (128, 512), (129, 640),
+    (300, 64), (257, 1001), (1000, 1024)])
+def test_quantisation_bytes(shape, block_rows, dtype):
+    x = matrix(*shape, seed=5, dtype=dtype, device="cuda")
+    b = F.quantize_fp8_blocks(x, block_rows)
+    equal_blocks(b, x, block_rows)
+    for out in DTYPES:
+        want = torch_ref.dequantize_fp8_blocks(b.q.cpu(), b.scale.cpu(), shape[1],
+                                               block_rows, out)
+        assert torch.equal(F.dequantize_fp8_blocks(b, out).cpu(), want)
+
+
+@gpu
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantisation_of_extremes(block_rows):
+    x = torch.randn(140, 300)
+    x[0] = 0
+    x[1, :128] = 0
+    x[2, 5] = float("inf")
+    x[3, 130] = float("nan")
+    x[4] = float("-inf")
+    x[5] = 3.0e38
+    x[6] = 1e-42  # not a normal number
+    x[7] = 2.0 ** -126
+    x[8, 0], x[8, 1] = 1e30, 1e-30
+    x[9] = torch.where(torch.rand(300) < 0.5, 17.0, 19.0)  # ties
+    x[10] = -0.0
+    equal_blocks(F.quantize_fp8_blocks(x.cuda(), block_rows), x, block_rows)
+    if block_rows == 1:
+        # rows do not affect each other
+        alone = F.quantize_fp8_blocks(x[20:21].cuda())
+        assert torch.equal(F.quantize_fp8_blocks(x.cuda()).q[20:21], alone.q)
+        back = F.dequantize_fp8_blocks(F.quantize_fp8_blocks(x.cuda())).cpu()
+        assert back[2, 5].isnan() and back[2, :5].isfinite().all()
+        assert back[4].isnan().all() and not back[0].any()
+
+
+@gpu
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantisation_of_views(block_rows):
+    base = matrix(200, 700, 3, torch.bfloat16, "cuda")
+    for x in (base[:, 1:400], base[::2, 8:520], base[:, 3:4], base.t(),
+              base[5:6].expand(64, 700), base.t()[10:20], base[:, ::2]):
+        equal_blocks(F.quantize_fp8_blocks(x, block_rows), x, block_rows)
+
+
+# -- GPU: products ---------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("blocks", [(1, 128), (1, 1), (128, 128), (128, 1)])
+@pytest.mark.parametrize("m,n,k", [
+    (1, 1, 1), (1, 1024, 3136), (2, 17, 130), (16, 16, 128), (17, 33, 257),
+    (31, 100, 64), (128, 128, 128), (129, 127, 129), (200, 515, 1000),
+    (1037, 517, 391), (600, 1024, 1500), (2100, 300, 700)])
+def test_product(m, n, k, blocks, dtype):
+    a = F.quantize_fp8_blocks(matrix(m, k, 1, device="cuda"), blocks[0])
+    b = F.quantize_fp8_blocks(matrix(n, k, 2, device="cuda"), blocks[1])
+    bias = matrix(1, n, 3, dtype, "cuda")[0]
+    av = F.dequantize_fp8_blocks(a).double().cpu()
+    bv = F.dequantize_fp8_blocks(b).double().cpu()
+    if dtype == torch.float16:  # keep results in its range
+        a = a._replace(scale=torch.where(a.scale > 20, a.scale - 8, a.scale))
+        av = F.dequantize_fp8_blocks(a).double().cpu()
+    z, size = av @ bv.t(), av.abs() @ bv.abs().t()
+    near(F.matmul_fp8_blocks(a, b, out_dtype=dtype), z, tol(k, size, z, dtype))
+    z, size = z + bias.double().cpu(), size + bias.double().cpu().abs()
+    near(F.matmul_fp8_blocks(a, b, bias, True, dtype), z.clamp(min=0),
+         tol(k + 1, size, z, dtype))
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 40, 700])
+def test_product_of_nan_stays_in_its_row(m):
+    x, w = matrix(m, 300, 1, device="cuda"), matrix(600, 300, 2, device="cuda")
+    x[m // 2, 7] = float("nan")
+    y = F.matmul_fp8_blocks(F.quantize_fp8_blocks(x), F.quantize_fp8_blocks(w, 128),
+                            relu=True)
+    bad = y.isnan().all(1)
+    assert bad[m // 2] and int(bad.sum()) == 1
+    assert int(y.isnan().sum()) == 600
+
+
+# -- GPU: the linear layer --------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtypes", [
+    (torch.float32,) * 3, (torch.bfloat16,) * 3, (torch.float16,) * 3,
+    (torch.bfloat16, torch.float32, torch.float32)])
+@pytest.mark.parametrize("m,n,k", [
+    (1, 1, 1), (1, 1024, 200), (5, 6, 512), (33, 130, 129), (256, 96, 300),
+    (700, 257, 385), (1300, 128, 256), (3000, 40, 72), (1025, 513, 640)])
+def test_linear(m, n, k, dtypes, relu):
+    x = (0.25 * matrix(m, k, 1)).clamp(-8, 8).to(dtypes[0]).cuda().requires_grad_()
+    w = (torch.rand(n, k, generator=torch.Generator().manual_seed(2)) - 0.5)
+    w = w.to(dtypes[1]).cuda().requires_grad_()
+    b = matrix(1, n, 3)[0].clamp(-1, 1).to(dtypes[2]).cuda().requires_grad_()
+    dy = (0.1 * matrix(m, n, 4)).clamp(-2, 2).to(dtypes[0]).cuda()
+    y = F.linear_fp8_blocks(x, w, b, relu)
+    assert y.dtype == x.dtype
+    y.backward(dy)
+    assert (x.grad.dtype, w.grad.dtype, b.grad.dtype) == dtypes
+    check_linear(x, w, b, dy, y, x.grad, w.grad, b.grad, relu)
+    # serving the same weight, laid out once
+    with torch.no_grad():
+        served = F.linear_fp8_blocks(x, F.quantize_fp8_blocks(w, 128), b, relu)
+        plain = F.linear_fp8_blocks(x, w, b, relu)
+    xh, wh = held(x), held(w, 128)
+    z = xh @ wh.t() + b.detach().double().cpu()
+    size = xh.abs() @ wh.abs().t() + b.detach().double().cpu().abs()
+    for out in (served, plain):
+        near(out, z.clamp(min=0) if relu else z, tol(k + 1, size, z, dtypes[0]))
+
+
+@gpu
+def test_linear_gradients_against_differences():
+    """Whole numbers up to 15 are held exactly beside each other, and the layer
+    is linear in each argument: a difference of 1 in one place is its gradient,
+    and sums of whole numbers in fp32 are exact."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randint(-7, 8, (6, 140), generator=g).float().cuda().requires_grad_()
+    w = torch.randint(-7, 8, (9, 140), generator=g).float().cuda().requires_grad_()
+    b = torch.randint(-7, 8, (9,), generator=g).float().cuda().requires_grad_()
+    dy = torch.randint(-7, 8, (6, 9), generator=g).float().cuda()
+    loss = lambda: (F.linear_fp8_blocks(x, w, b) * dy).sum()  # noqa: E731
+    loss().backward()
+    with torch.no_grad():
+        base = loss()
+        for t, places in ((x, [(0, 0), (3, 127), (5, 139)]),
+                          (w, [(0, 5), (8, 128), (4, 139)]), (b, [(0,), (8,)])):
+            for at in places:
+                t[at] += 1
+                assert float(loss() - base) == float(t.grad[at])
+                t[at] -= 1
+
+
+@gpu
+def test_linear_parts_of_the_gradient():
+    x = matrix(300, 200, 1, torch.bfloat16, "cuda")
+    w = matrix(70, 200, 2, torch.bfloat16, "cuda")
+    b = matrix(1, 70, 3, torch.bfloat16, "cuda")[0]
+    dy = matrix(300, 70, 4, torch.bfloat16, "cuda")
+    whole = [t.clone().requires_grad_() for t in (x, w, b)]
+    all_grads = torch.autograd.grad(
+        F.linear_fp8_blocks(*whole, relu=True), whole, dy)
+    for want in ([0], [1], [2], [0, 2], [1, 2], [0, 1]):
+        args = [t.clone().requires_grad_(i in want) for i, t in enumerate((x, w, b))]
+        grads = torch.autograd.grad(F.linear_fp8_blocks(*args, relu=True),
+                                    [args[i] for i in want], dy)
+        for i, g in zip(want, grads):
+            assert torch.equal(g, all_grads[i])
+    # without a bias, and with a gradient that is one number spread out
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = F.linear_fp8_blocks(xs, ws)
+    y.sum().backward()
+    one = torch.ones_like(y)
+    check_linear(xs, ws, None, one, y, xs.grad, ws.grad, None, False)
+
+
+@gpu
+def test_linear_shapes_and_views():
+    base = matrix(50, 260, 1, torch.bfloat16, "cuda")
+    w = matrix(40, 260, 2, torch.bfloat16, "cuda")
+    want = F.linear_fp8_blocks(base, w)
+    assert torch.equal(F.linear_fp8_blocks(base.view(5, 10, 260), w),
+                       want.view(5, 10, 40))
+    assert torch.equal(F.linear_fp8_blocks(base[7], w), want[7])
+    assert torch.equal(F.linear_fp8_blocks(base.t().contiguous().t(), w), want)
+    wide = torch.cat([base, base], 1)
+    assert torch.equal(F.linear_fp8_blocks(wide[:, 260:], w), want)
+    assert torch.equal(F.linear_fp8_blocks(base, w.t().contiguous().t()), want)
+    x = base.clone().view(5, 10, 260).transpose(0, 1).requires_grad_()
+    F.linear_fp8_blocks(x, w).sum().backward()
+    assert x.grad.shape == x.shape
+
+
+@gpu
+def test_kept_in_8_bits():
+    """What waits for the backward pass is x in 8 bits and the weight's copy."""
+    x = torch.randn(4096, 2048, device="cuda", dtype=torch.bfloat16)
+    x.requires_grad_()
+    w = torch.randn(256, 2048, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = F.linear_fp8_blocks(x, w, relu=True)
+    kept = torch.cuda.memory_allocated() - before - y.numel() * 2
+    # x, its scales, the transposed weight, the bits; and the allocator's rounding
+    assert kept <= 4096 * (2048 + 16) + 2048 * 256 * 2 + 4096 * 32 + 8 * 2 ** 20 / 4
+
+
+@gpu
+def test_same_bits_every_time():
+    x = matrix(3000, 500, 1, torch.bfloat16, "cuda").requires_grad_()
+    w = matrix(300, 500, 2, torch.bfloat16, "cuda").requires_grad_()
+    b = matrix(1, 300, 3, torch.bfloat16, "cuda")[0].requires_grad_()
+    dy = matrix(3000, 300, 4, torch.bfloat16, "cuda")
+    one = lambda: torch.autograd.grad(  # noqa: E731
+        F.linear_fp8_blocks(x, w, b, True), (x, w, b), dy)
+    first = one()
+    for _ in range(3):
+        assert all(torch.equal(p, q) for p, q in zip(one(), first))
+
+
+@gpu
+def test_on_another_stream():
+    x, w = matrix(900, 300, 1, device="cuda"), matrix(200, 300, 2, device="cuda")
+    want = F.linear_fp8_blocks(x, w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        big = torch.randn(4096, 4096, device="cuda")
+        for _ in range(4):
+            big = big @ big * 1e-4
+        late = x + 0 * big[0, 0]  # x, but only when the products are done
+        got = F.linear_fp8_blocks(late, w)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_captured_step_replays():
+    """Two graphs of a training step, replayed in turn with eager work between,
+    give what the eager step gives on the same inputs."""
+    shapes = [(256, 200, 300), (1500, 130, 257)]
+    graphs = []
+    for m, n, k in shapes:
+        x = matrix(m, k, 1, torch.bfloat16, "cuda").requires_grad_()
+        w = matrix(n, k, 2, torch.bfloat16, "cuda").requires_grad_()
+        b = matrix(1, n, 3, torch.bfloat16, "cuda")[0].requires_grad_()
+        dy = matrix(m, n, 4, torch.bfloat16, "cuda")
+        step = lambda x=x, w=w, b=b, dy=dy: torch.autograd.grad(  # noqa: E731
+            F.linear_fp8_blocks(x, w, b, True), (x, w, b), dy)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        graphs.append((graph, outs, x, step))
+    for i in range(4):
+        for graph, outs, x, step in graphs:
+            with torch.no_grad():
+                x.copy_(matrix(*x.shape, 10 + i, torch.bfloat16, "cuda"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(outs, step()))
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """A matrix of more than 2^31 values: the last rows as by themselves."""
+    rows, cols = 2 ** 20 + 3, 2050
+    x = torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16)
+    tail = matrix(200, cols, 7, torch.bfloat16, "cuda")
+    x[-200:] = tail
+    w = matrix(20, cols, 8, torch.bfloat16, "cuda")
+    got, want = F.quantize_fp8_blocks(x), F.quantize_fp8_blocks(tail)
+    assert torch.equal(got.q[-200:], want.q)
+    assert torch.equal(got.scale[-200:], want.scale)
+    wb = F.quantize_fp8_blocks(w, 128)
+    y = F.matmul_fp8_blocks(got, wb, out_dtype=torch.float32)
+    z = held(tail) @ held(w, 128).t()
+    size = held(tail).abs() @ held(w, 128).abs().t()
+    near(y[-200:], z, tol(cols, size, z, torch.float32))
+    assert not y[:-200].any()
+    back = F.dequantize_fp8_blocks(got, torch.bfloat16)
+    assert torch.equal(back[-200:], F.dequantize_fp8_blocks(want, torch.bfloat16))
+    del back, y
+    dy = torch.zeros(rows, 20, device="cuda", dtype=torch.bfloat16)
+    dy[-200:] = matrix(200, 20, 9, torch.bfloat16, "cuda")
+    w.requires_grad_()
+    F.linear_fp8_blocks(x, w).backward(dy)
+    g = held(dy[-200:])
+    want = g.t() @ held(tail)
+    near(w.grad, want, tol(200, g.abs().t() @ held(tail).abs(), want, torch.bfloat16))

@@ -1,0 +1,282 @@
+"""Layer norm (ops/functional.py) against a plain 64-bit form.
+
+Tolerances, fixed beforehand.  fp32 sums of C terms in any order are off by at
+most C 2^-24 of the sum of magnitudes.  With A = max |x| of a row and std its
+sqrt(var + eps): the mean is off by C 2^-24 A, a distance by that and 2^-24 A,
+so h = (x - mean) / std by (C + 4) 2^-24 A / std and, through the variance (a
+sum of C squares, then a root and a product), by (C + 8) 2^-24 |h| more.  The
+worst case of every sum at once is far from what happens, and these bounds are
+still some 1e-3 at most here.  The backward pass adds two means of C terms of
+|g| and |g h|; every result ends with its own rounding, eps / 2."""
+
+import pytest
+import torch
+
+from rainbowiqn_amd.ops import functional as F
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def plain(x, w, b, eps, dy=None):
+    """y, dx, dw, db and bounds for them, in 64 bits on the CPU."""
+    x = x.detach().double().cpu()
+    c = x.shape[1]
+    w = torch.ones(c).double() if w is None else w.detach().double().cpu()
+    b = torch.zeros(c).double() if b is None else b.detach().double().cpu()
+    d = x - x.mean(1, keepdim=True)
+    std = ((d * d).mean(1, keepdim=True) + eps).sqrt()
+    h = d / std
+    eh = (c + 4) * U * x.abs().amax(1, keepdim=True) / std + (c + 8) * U * h.abs()
+    out = {"y": (h * w + b, eh * w.abs() + 4 * U * ((h * w).abs() + b.abs()))}
+    if dy is not None:
+        dy = dy.detach().double().cpu()
+        g = dy * w
+        c2 = (g * h).mean(1, keepdim=True)
+        dx = (g - g.mean(1, keepdim=True) - h * c2) / std
+        mag = g.abs() + g.abs().mean(1, keepdim=True) + h.abs() * (
+            g * h).abs().mean(1, keepdim=True)
+        e = (c + 12) * U * mag + eh * c2.abs() + h.abs() * (
+            g.abs() * eh).mean(1, keepdim=True)
+        rel_std = (c + 8) * U + ((c + 4) * U * x.abs().amax(1, keepdim=True) / std) ** 2
+        out["dx"] = (dx, e / std + rel_std * dx.abs())
+        r = x.shape[0]
+        out["dw"] = ((dy * h).sum(0), (r + 4) * U * (dy * h).abs().sum(0)
+                     + (dy.abs() * eh).sum(0))
+        out["db"] = (dy.sum(0), (r + 4) * U * dy.abs().sum(0))
+    return out
+
+
+def near(got, want, bound):
+    assert got.shape == want.shape
+    tiny = torch.finfo(got.dtype).smallest_normal
+    off = ((got.detach().double().cpu() - want).abs() - bound
+           - torch.finfo(got.dtype).eps / 2 * (want.abs() + bound) - tiny)
+    assert bool((off <= 0).all()), float(off.max())
+
+
+def inputs(r, c, dtype, wdtype, device, offset=0.3):
+    g = torch.Generator().manual_seed(r * 10007 + c)
+    x = (torch.randn(r, c, generator=g) + offset) * torch.exp(
+        torch.randn(r, 1, generator=g))
+    w = 1 + 0.5 * torch.randn(c, generator=g)
+    b = torch.randn(c, generator=g)
+    dy = torch.randn(r, c, generator=g)
+    return (x.to(dtype).to(device).requires_grad_(),
+            w.to(wdtype).to(device).requires_grad_(),
+            b.to(wdtype).to(device).requires_grad_(), dy.to(dtype).to(device))
+
+
+def step(x, w, b, dy, eps=1e-5):
+    y = F.layer_norm(x, w, b, eps)
+    leaves = [t for t in (x, w, b) if t is not None]
+    grads = dict(zip([n for n, t in zip(("dx", "dw", "db"), (x, w, b))
+                      if t is not None], torch.autograd.grad(y, leaves, dy)))
+    return {"y": y, **grads}
+
+
+SHAPES = [(1, 1), (1, 3136), (3, 2), (5, 8), (7, 511), (64, 512), (33, 513),
+          (130, 1024), (129, 1537), (2050, 200), (257, 3136), (50, 4096),
+          (9, 4097), (300, 5000), (2, 40000)]
+TYPES = [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
+         (torch.bfloat16, torch.float32), (torch.float16, torch.float16),
+         (torch.float16, torch.float32)]
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (7, 33), (20, 300)])
+def test_cpu(shape):
+    x, w, b, dy = inputs(*shape, torch.float32, torch.float32, "cpu")
+    got = step(x, w, b, dy)
+    for name, (want, bound) in plain(x, w, b, 1e-5, dy).items():
+        near(got[name], want, bound)
+
+
+def test_formula_against_differences():
+    """The plain form's gradients against central differences in 64 bits: off by
+    h^2 (1e-10) of third derivatives of order 10 and 1e-16 / h of the loss."""
+    x, w, b, dy = inputs(3, 17, torch.float32, torch.float32, "cpu")
+    out = plain(x, w, b, 1e-5, dy)
+    args = [t.detach().double() for t in (x, w, b)]
+    loss = lambda: float((plain(*args, 1e-5)["y"][0] * dy.double()).sum())  # noqa: E731
+    for t, name, places in ((args[0], "dx", [(0, 0), (1, 9), (2, 16)]),
+                            (args[1], "dw", [(0,), (16,)]),
+                            (args[2], "db", [(0,), (16,)])):
+        for at in places:
+            keep = float(t[at])
+            t[at] = keep + 1e-5
+            up = loss()
+            t[at] = keep - 1e-5
+            down = loss()
+            t[at] = keep
+            assert abs((up - down) / 2e-5 - float(out[name][0][at])) < 1e-7
+
+
+@gpu
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_step(shape, types):
+    x, w, b, dy = inputs(*shape, *types, "cuda")
+    got = step(x, w, b, dy)
+    for name, (want, bound) in plain(x, w, b, 1e-5, dy).items():
+        near(got[name], want, bound)
+    assert got["dw"].dtype == types[1] and got["dx"].dtype == types[0]
+    with torch.no_grad():
+        assert torch.equal(F.layer_norm(x, w, b), got["y"])
+
+
+@gpu
+@pytest.mark.parametrize("which", [(0, 0), (1, 0), (0, 1)])
+@pytest.mark.parametrize("cols", [300, 4500])
+def test_without_weight_or_bias(cols, which):
+    x, w, b, dy = inputs(40, cols, torch.float32, torch.float32, "cuda")
+    w, b = w if which[0] else None, b if which[1] else None
+    got = step(x, w, b, dy)
+    want = plain(x, w, b, 1e-5, dy)
+    for name in got:
+        near(got[name], *want[name])
+
+
+@gpu
+@pytest.mark.parametrize("cols", [64, 3136, 4100])
+def test_rows_that_are_hard(cols):
+    """A large offset keeps its digits, equal values give the bias, and what is
+    not finite stays in its row."""
+    x, w, b, dy = inputs(8, cols, torch.float32, torch.float32, "cuda")
+    with torch.no_grad():
+        x[1] += 1000.0
+        x[2] = 5.0
+        x[3, 7] = float("inf")
+        x[4, 9] = float("nan")
+        x[5] = 0.0
+        x[6] *= 1e15
+    got = step(x, w, b, dy)
+    fine = [0, 1, 2, 5, 6, 7]
+    want = plain(x[fine], w, b, 1e-5, dy[fine])
+    for name in ("y", "dx"):
+        near(got[name][fine], *want[name])
+        assert got[name][3:5].isnan().all()
+    assert torch.equal(got["y"][2], b.detach())
+    assert got["db"].isfinite().all()
+
+
+@gpu
+@pytest.mark.parametrize("cols", [504, 4600])
+def test_views(cols):
+    base = torch.randn(60, 2 * cols + 16, device="cuda").to(torch.bfloat16)
+    w = torch.randn(cols, device="cuda").to(torch.bfloat16)
+    for x in (base[:, 1:cols + 1], base[::3, 8:cols + 8], base[:, :2 * cols:2],
+              base[:1, :cols].expand(17, cols), base[:, :cols].t()[:60].t()):
+        want = F.layer_norm(x.contiguous(), w[:x.shape[1]].contiguous())
+        assert torch.equal(F.layer_norm(x, w[:x.shape[1]].contiguous()), want)
+    x = base[:, 3:cols + 3].detach().requires_grad_()
+    y = F.layer_norm(x.view(5, 12, cols) if x.is_contiguous() else x, w)
+    y.sum().backward()  # a gradient that is one number spread out
+    near(x.grad, *plain(x, w, None, 1e-5, torch.ones_like(y))["dx"])
+    # weights that are not 16-byte aligned
+    w1 = torch.randn(cols + 1, device="cuda")[1:]
+    x = base[:, :cols]
+    near(F.layer_norm(x, w1), *plain(x, w1, None, 1e-5)["y"])
+    # leading dimensions
+    x3 = base[:, :cols].reshape(3, 4, 5, cols)
+    assert torch.equal(F.layer_norm(x3, w).view(60, cols), F.layer_norm(x, w))
+    assert torch.equal(F.layer_norm(x[7], w), F.layer_norm(x, w)[7])
+
+
+def refusals(device):
+    x, w = torch.randn(4, 30, device=device), torch.randn(30, device=device)
+    for call in (lambda: F.layer_norm(x, w[:29]),
+                 lambda: F.layer_norm(x, None, w[:29]),
+                 lambda: F.layer_norm(x, w.view(1, 30)),
+                 lambda: F.layer_norm(x, w, eps=-1.0),
+                 lambda: F.layer_norm(x, w, eps=float("nan")),
+                 lambda: F.layer_norm(x, w.bfloat16()),
+                 lambda: F.layer_norm(x.bfloat16(), w, w.bfloat16()),
+                 lambda: F.layer_norm(x.long(), w),
+                 lambda: F.layer_norm(x[:, :0]),
+                 lambda: F.layer_norm(x[0, 0])):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def test_refusals_cpu():
+    refusals("cpu")
+
+
+@gpu
+def test_refusals_gpu():
+    refusals("cuda")
+    x, w = torch.randn(4, 30, device="cuda"), torch.randn(60, device="cuda")
+    for call in (lambda: F.layer_norm(x, w.cpu()[:30]),
+                 lambda: F.layer_norm(x, w[::2])):
+        with pytest.raises(RuntimeError):
+            call()
+    x.requires_grad_()
+    y = F.layer_norm(x)
+    (g,) = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_no_rows(device):
+    x = torch.zeros(0, 40, device=device, requires_grad=True)
+    w = torch.ones(40, device=device, requires_grad=True)
+    y = F.layer_norm(x, w, w)
+    y.sum().backward()
+    assert y.shape == x.grad.shape == (0, 40) and not w.grad.any()
+
+
+@gpu
+def test_parts_of_the_gradient_and_same_bits():
+    x, w, b, dy = inputs(700, 1000, torch.bfloat16, torch.float32, "cuda")
+    whole = torch.autograd.grad(F.layer_norm(x, w, b), (x, w, b), dy)
+    for want in ([0], [1], [2], [0, 2], [1, 2]):
+        args = [t.detach().clone().requires_grad_(i in want)
+                for i, t in enumerate((x, w, b))]
+        grads = torch.autograd.grad(F.layer_norm(*args), [args[i] for i in want], dy)
+        for i, g in zip(want, grads):
+            assert torch.equal(g, whole[i])
+
+
+@gpu
+def test_captured_step_replays():
+    graphs = []
+    for shape in ((256, 3136), (40, 5000)):
+        x, w, b, dy = inputs(*shape, torch.bfloat16, torch.bfloat16, "cuda")
+        one = lambda x=x, w=w, b=b, dy=dy: list(step(x, w, b, dy).values())  # noqa: E731
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            one()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = one()
+        graphs.append((graph, outs, x, one))
+    for i in range(4):
+        for graph, outs, x, one in graphs:
+            with torch.no_grad():
+                x.copy_(torch.randn(x.shape, device="cuda"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(outs, one()))
+
+
+@gpu
+def test_offsets_past_32_bits():
+    rows, cols = 2 ** 20 + 3, 2056
+    x = torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16)
+    tail, w, b, dy = inputs(50, cols, torch.bfloat16, torch.bfloat16, "cuda")
+    x[-50:] = tail.detach()
+    x.requires_grad_()
+    y = F.layer_norm(x, w, b)
+    assert torch.equal(y[-50:], F.layer_norm(tail, w, b))
+    g = torch.zeros_like(y)
+    g[-50:] = dy
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    got = {"dx": dx[-50:], "dw": dw, "db": db}
+    want = plain(tail, w, b, 1e-5, dy)
+    for name in got:
+        near(got[name], *want[name])
+    assert not dx[:-50].any()
