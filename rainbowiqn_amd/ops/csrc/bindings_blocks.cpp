@@ -485,7 +485,7 @@ class NormFn : public torch::autograd::Function<NormFn> {
             if (dw.defined()) dw.zero_();
             if (db.defined()) db.zero_();
         } else {
-            const int groups = row_groups(R, 4, 512);
+            const int groups = riqn_norm_groups((int)R, (int)C);
             Tensor part;
             if (need & 6) part = torch::empty({groups, 2, C}, floats_on(x));
             launched(riqn_norm_bwd(

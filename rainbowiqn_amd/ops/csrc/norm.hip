@@ -9,19 +9,22 @@
 // it in fp32, rounded once on the way out.
 //
 // Both passes are bound by memory: forward reads x and writes y, backward
-// reads x and dy and writes dx.  Up to 4096 columns one wave holds a row in
-// registers (8 neighbours a lane, NV times), so a row is read once and no
-// wave waits for another; longer rows are walked over again by a workgroup,
-// out of the cache.
+// reads x and dy and writes dx.  Rows of up to 4096 columns stay in registers
+// between the sums and the result, 8 neighbours a lane and NV times that, so
+// they are read once.  A team of 1 wave (up to 1024 columns) or 4 waves takes
+// 4 rows at a time: 4 rows of loads in flight, one exchange of sums through
+// LDS for all of them, and the weights stay in registers for the next 4.
+// Longer rows are walked over again by a workgroup, out of the cache.
 //
-// dw and db: each wave adds its rows up in registers, the workgroup's waves
-// add theirs in LDS one after the other, and workgroup g writes part[g]; a
-// second kernel adds the parts.  No atomics: the same inputs give the same
-// bits.
+// dw and db: a lane adds its columns up in registers over all its rows,
+// workgroup g writes part[g], and a second kernel adds the parts.  No atomics:
+// the same inputs give the same bits.
 #include "common.h"
 #include "riqn_kernels.h"
 
 namespace {
+
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
 struct bf16_t { unsigned short v; };
 struct fp16_t { _Float16 v; };
@@ -35,32 +38,76 @@ template <> DEV bf16_t from_f<bf16_t>(float x) {
 }
 template <> DEV fp16_t from_f<fp16_t>(float x) { return fp16_t{(_Float16)x}; }
 
-template <typename T, bool VEC> struct Pack8;
-template <typename T> struct alignas(16) Pack8<T, true> { T t[8]; };
-template <typename T> struct Pack8<T, false> { T t[8]; };
+template <typename T> struct Bits { using type = unsigned short; };
+template <> struct Bits<float> { using type = uint32_t; };
 
-// 8 neighbours from column `col`, zeros behind column C.  VEC: rows are
-// 16-byte aligned and C is a multiple of 8.
-template <typename T, bool VEC>
-DEV Pack8<T, VEC> load8(const T* p, int col, int C) {
-    Pack8<T, VEC> v;
-    if (col + 8 <= C) {
-        v = *(const Pack8<T, VEC>*)(p + col);
+// 8 values as they lie in memory.  Kept as whole registers: as single 16-bit
+// values the compiler gives each a register of its own.
+template <typename T>
+struct Pack8 {
+    static constexpr int WORDS = 2 * sizeof(T);
+    uint32_t w[WORDS];
+    DEV float get(int i) const {
+        if (sizeof(T) == 4) return __uint_as_float(w[i]);
+        const uint32_t u = w[i >> 1];
+        const unsigned short h = (unsigned short)(i & 1 ? u >> 16 : u);
+        return to_f(__builtin_bit_cast(T, (typename Bits<T>::type)h));
+    }
+    DEV void set(int i, float v) {
+        const auto bits = __builtin_bit_cast(typename Bits<T>::type, from_f<T>(v));
+        if (sizeof(T) == 4) w[i] = bits;
+        else if (i & 1) w[i >> 1] |= (uint32_t)bits << 16;
+        else w[i >> 1] = bits;
+    }
+};
+
+// 8 neighbours from column `col`.  Behind column C: zeros where ZERO is set,
+// anything finite or from the same row otherwise.  VEC: rows are 16-byte
+// aligned and C is a multiple of 8; then the load is unconditional (from the
+// row's last 8 columns), as a branch around each would keep them apart.
+template <typename T, bool VEC, bool ZERO>
+DEV Pack8<T> load8(const T* p, int col, int C) {
+    Pack8<T> v;
+    if (VEC) {
+        const uint32_t* q = (const uint32_t*)(p + min(col, C - 8));
+        #pragma unroll
+        for (int i = 0; i < Pack8<T>::WORDS; i += 4)
+            *(u32x4*)&v.w[i] = *(const u32x4*)(q + i);
+        if (ZERO) {
+            #pragma unroll
+            for (int i = 0; i < Pack8<T>::WORDS; ++i)
+                v.w[i] = col < C ? v.w[i] : 0;
+        }
+    } else if (col + 8 <= C) {
+        __builtin_memcpy(v.w, p + col, sizeof(v.w));
     } else {
         #pragma unroll
         for (int i = 0; i < 8; ++i)
-            v.t[i] = (!VEC && col + i < C) ? p[col + i] : T{};
+            v.set(i, col + i < C ? to_f(p[col + i]) : 0.0f);
     }
     return v;
 }
+template <typename T>
+DEV Pack8<T> all8(float x) {
+    Pack8<T> v;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) v.set(i, x);
+    return v;
+}
 template <typename T, bool VEC>
-DEV void store8(T* p, int col, int C, const Pack8<T, VEC>& v) {
+DEV void store8(T* p, int col, int C, const Pack8<T>& v) {
     if (col + 8 <= C) {
-        *(Pack8<T, VEC>*)(p + col) = v;
+        if (VEC) {
+            #pragma unroll
+            for (int i = 0; i < Pack8<T>::WORDS; i += 4)
+                *(u32x4*)((uint32_t*)(p + col) + i) = *(const u32x4*)&v.w[i];
+        } else {
+            __builtin_memcpy(p + col, v.w, sizeof(v.w));
+        }
     } else if (!VEC) {
         #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (col + i < C) p[col + i] = v.t[i];
+            if (col + i < C) p[col + i] = from_f<T>(v.get(i));
     }
 }
 
@@ -97,55 +144,112 @@ struct NormFwd {
     float eps;
 };
 
-template <typename T, typename W, int NV, bool VEC>
+constexpr int RB = 4;  // rows a team takes at a time
+
+// Sums of N values over a team of TW waves, in every lane.  `lds` is
+// [2][4][N] floats; `turn` alternates, so that one barrier a sum is enough:
+// what a slow wave still reads is not written before the next barrier.
+template <int TW, int N>
+DEV void team_sum(float (&v)[N], float* lds, int& turn) {
+    #pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    if (TW == 1) return;
+    float* s = lds + turn * 4 * N;
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) s[(threadIdx.x >> 6) * N + i] = v[i];
+    }
+    __syncthreads();
+    #pragma unroll
+    for (int i = 0; i < N; ++i)
+        v[i] = (s[i] + s[N + i]) + (s[2 * N + i] + s[3 * N + i]);
+}
+
+// Makes the compiler take a loaded value for a new one: what was derived from
+// it before a sum is derived again after it.  Kept instead, the fp32 values
+// of 4 rows would take twice the registers and halve the waves in flight.
+template <typename T>
+DEV void forget(Pack8<T>& p) {
+    #pragma unroll
+    for (int i = 0; i < Pack8<T>::WORDS; ++i) asm volatile("" : "+v"(p.w[i]));
+}
+
+template <typename T, typename W, int TW, int NV, bool VEC>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(NormFwd a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= a.R) return;
-    const T* x = (const T*)a.x + r * a.ldx;
-    float v[NV][8];
-    float s = 0.0f;
+    __shared__ float lds[2 * 4 * RB];
+    const int t = threadIdx.x % (64 * TW);  // place in the team
+    constexpr int TEAMS = 4 / TW;
+    int turn = 0;
+    Pack8<W> w[NV], b[NV];
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const auto p = load8<T, VEC>(x, (i * 64 + lane) * 8, a.C);
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[i][j] = to_f(p.t[j]);
-            s += v[i][j];
-        }
+        const int col = (i * 64 * TW + t) * 8;
+        w[i] = a.w ? load8<W, VEC, false>((const W*)a.w, col, a.C) : all8<W>(1.0f);
+        b[i] = a.b ? load8<W, VEC, false>((const W*)a.b, col, a.C) : all8<W>(0.0f);
     }
-    const float mean = wave_sum(s) / a.C;
-    s = 0.0f;
-    #pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    for (int64_t r0 = ((int64_t)blockIdx.x * TEAMS + threadIdx.x / (64 * TW)) * RB;
+         r0 < a.R; r0 += (int64_t)gridDim.x * TEAMS * RB) {
+        Pack8<T> x[RB][NV];
         #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            // what is not there counts for nothing
-            v[i][j] = (i * 64 + lane) * 8 + j < a.C ? v[i][j] - mean : 0.0f;
-            s += v[i][j] * v[i][j];
+        for (int k = 0; k < RB; ++k) {
+            // rows behind the last one are read as the last
+            const int64_t r = min(r0 + k, (int64_t)a.R - 1);
+            #pragma unroll
+            for (int i = 0; i < NV; ++i)
+                x[k][i] = load8<T, VEC, true>((const T*)a.x + r * a.ldx,
+                                        (i * 64 * TW + t) * 8, a.C);
         }
-    }
-    const float rstd = 1.0f / sqrtf(wave_sum(s) / a.C + a.eps);
-    if (a.mean && lane == 0) {
-        a.mean[r] = mean;
-        a.rstd[r] = rstd;
-    }
-    T* y = (T*)a.y + r * a.C;
-    #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int col = (i * 64 + lane) * 8;
-        Pack8<W, VEC> w, b;
-        if (a.w) w = load8<W, VEC>((const W*)a.w, col, a.C);
-        if (a.b) b = load8<W, VEC>((const W*)a.b, col, a.C);
-        Pack8<T, VEC> o;
+        float mean[RB], rstd[RB];
         #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float z = v[i][j] * rstd;
-            if (a.w) z *= to_f(w.t[j]);
-            if (a.b) z += to_f(b.t[j]);
-            o.t[j] = from_f<T>(z);
+        for (int k = 0; k < RB; ++k) {
+            mean[k] = 0.0f;
+            #pragma unroll
+            for (int i = 0; i < NV; ++i)
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) mean[k] += x[k][i].get(j);
         }
-        store8<T, VEC>(y, col, a.C, o);
+        team_sum<TW, RB>(mean, lds, turn);
+        #pragma unroll
+        for (int k = 0; k < RB; ++k) {
+            mean[k] /= a.C;
+            #pragma unroll
+            for (int i = 0; i < NV; ++i) forget(x[k][i]);
+            rstd[k] = 0.0f;
+            #pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float d = x[k][i].get(j) - mean[k];
+                    // what is not there counts for nothing
+                    if ((i * 64 * TW + t) * 8 + (VEC ? 0 : j) < a.C)
+                        rstd[k] += d * d;
+                }
+            }
+        }
+        team_sum<TW, RB>(rstd, lds, turn);
+        #pragma unroll
+        for (int k = 0; k < RB; ++k) {
+            rstd[k] = 1.0f / sqrtf(rstd[k] / a.C + a.eps);
+            const int64_t r = r0 + k;
+            if (r >= a.R) continue;
+            #pragma unroll
+            for (int i = 0; i < NV; ++i) forget(x[k][i]);
+            if (a.mean && t == 0) {
+                a.mean[r] = mean[k];
+                a.rstd[r] = rstd[k];
+            }
+            #pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                Pack8<T> o;
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float h = (x[k][i].get(j) - mean[k]) * rstd[k];
+                    o.set(j, h * w[i].get(j) + b[i].get(j));
+                }
+                store8<T, VEC>((T*)a.y + r * a.C, (i * 64 * TW + t) * 8, a.C, o);
+            }
+        }
     }
 }
 
@@ -187,79 +291,116 @@ struct NormBwd {
     int R, C;
 };
 
-template <typename T, typename W, int NV, bool VEC>
-__global__ __launch_bounds__(256) void norm_bwd_kernel(NormBwd a) {
-    extern __shared__ float lds[];  // [2][C] where part is asked for
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// 2 waves a SIMD: held to 3 the compiler spills, and [32768, 3136] in bf16
+// takes 165 us instead of 136 with the adding up of the parts (the bytes
+// alone take 121 at the rate of a large copy).
+template <typename T, typename W, int TW, int NV, bool VEC>
+__global__ __launch_bounds__(256, 2) void norm_bwd_kernel(NormBwd a) {
+    constexpr int TEAMS = 4 / TW;
+    // sums of the teams; where teams are waves, also their parts in turn
+    __shared__ float lds[TW == 1 ? 4 * NV * 512 : 2 * 2 * 4 * RB];
+    const int t = threadIdx.x % (64 * TW);
+    int turn = 0;
+    Pack8<W> w[NV];
     float dw[NV][8], db[NV][8];
     #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+        w[i] = a.w ? load8<W, VEC, false>((const W*)a.w, (i * 64 * TW + t) * 8, a.C)
+                   : all8<W>(1.0f);
         #pragma unroll
         for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.0f;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < a.R;
-         r += (int64_t)gridDim.x * 4) {
-        Pack8<T, VEC> x[NV], dy[NV];
-        #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = (i * 64 + lane) * 8;
-            x[i] = load8<T, VEC>((const T*)a.x + r * a.ldx, col, a.C);
-            dy[i] = load8<T, VEC>((const T*)a.dy + r * a.lddy, col, a.C);
-        }
-        const float mean = a.mean[r], rstd = a.rstd[r];
-        float s1 = 0.0f, s2 = 0.0f;
-        #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            Pack8<W, VEC> w;
-            if (a.w) w = load8<W, VEC>((const W*)a.w, (i * 64 + lane) * 8, a.C);
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                // behind column C dy is zero, so nothing is added there
-                const float d = to_f(dy[i].t[j]);
-                const float h = (to_f(x[i].t[j]) - mean) * rstd;
-                const float g = a.w ? d * to_f(w.t[j]) : d;
-                db[i][j] += d;
-                dw[i][j] += d * h;
-                s1 += g;
-                s2 += g * h;
-            }
-        }
-        if (!a.dx) continue;
-        const float c1 = wave_sum(s1) / a.C, c2 = wave_sum(s2) / a.C;
-        #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = (i * 64 + lane) * 8;
-            Pack8<W, VEC> w;
-            if (a.w) w = load8<W, VEC>((const W*)a.w, col, a.C);
-            Pack8<T, VEC> o;
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float d = to_f(dy[i].t[j]);
-                const float h = (to_f(x[i].t[j]) - mean) * rstd;
-                const float g = a.w ? d * to_f(w.t[j]) : d;
-                o.t[j] = from_f<T>(rstd * (g - c1 - h * c2));
-            }
-            store8<T, VEC>((T*)a.dx + r * a.C, col, a.C, o);
-        }
     }
-    if (!a.part) return;
-    for (int k = 0; k < 4; ++k) {
-        if (wave == k) {
+    for (int64_t r0 = ((int64_t)blockIdx.x * TEAMS + threadIdx.x / (64 * TW)) * RB;
+         r0 < a.R; r0 += (int64_t)gridDim.x * TEAMS * RB) {
+        Pack8<T> x[RB][NV], dy[RB][NV];
+        float mean[RB], rstd[RB];
+        #pragma unroll
+        for (int k = 0; k < RB; ++k) {
+            const int64_t r = min(r0 + k, (int64_t)a.R - 1);
+            mean[k] = a.mean[r];
+            rstd[k] = a.rstd[r];
+            #pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int col = (i * 64 * TW + t) * 8;
+                x[k][i] = load8<T, VEC, false>((const T*)a.x + r * a.ldx, col, a.C);
+                dy[k][i] = load8<T, VEC, true>((const T*)a.dy + r * a.lddy, col, a.C);
+            }
+        }
+        float s[2 * RB];  // sums of g and of g h
+        #pragma unroll
+        for (int k = 0; k < RB; ++k) {
+            s[2 * k] = s[2 * k + 1] = 0.0f;
+            const bool there = r0 + k < a.R;
             #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const int c = (i * 64 + lane) * 8 + j;
-                    if (c < a.C) {
-                        lds[c] = dw[i][j] + (k ? lds[c] : 0.0f);
-                        lds[a.C + c] = db[i][j] + (k ? lds[a.C + c] : 0.0f);
-                    }
+                    // behind column C dy is zero, so nothing is added there
+                    const float d = there ? dy[k][i].get(j) : 0.0f;
+                    const float h = (x[k][i].get(j) - mean[k]) * rstd[k];
+                    const float g = d * w[i].get(j);
+                    db[i][j] += d;
+                    dw[i][j] += d * h;
+                    // here, not at the loop's end with d and h of all rows
+                    // kept until then, which is what the compiler would do
+                    asm volatile("" : "+v"(db[i][j]), "+v"(dw[i][j]));
+                    s[2 * k] += g;
+                    s[2 * k + 1] += g * h;
                 }
             }
+            asm volatile("" : "+v"(s[2 * k]), "+v"(s[2 * k + 1]));
         }
-        __syncthreads();
+        if (!a.dx) continue;
+        team_sum<TW, 2 * RB>(s, lds, turn);
+        #pragma unroll
+        for (int k = 0; k < RB; ++k) {
+            const int64_t r = r0 + k;
+            if (r >= a.R) continue;
+            const float c1 = s[2 * k] / a.C, c2 = s[2 * k + 1] / a.C;
+            #pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                forget(x[k][i]);
+                forget(dy[k][i]);
+                Pack8<T> o;
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float d = dy[k][i].get(j);
+                    const float h = (x[k][i].get(j) - mean[k]) * rstd[k];
+                    const float g = d * w[i].get(j);
+                    o.set(j, rstd[k] * (g - c1 - h * c2));
+                }
+                store8<T, VEC>((T*)a.dx + r * a.C, (i * 64 * TW + t) * 8, a.C, o);
+            }
+        }
     }
+    if (!a.part) return;
     float* part = a.part + (int64_t)blockIdx.x * 2 * a.C;
-    for (int c = threadIdx.x; c < 2 * a.C; c += 256) part[c] = lds[c];
+    #pragma unroll
+    for (int which = 0; which < 2; ++which, part += a.C) {
+        if (TW == 1) {  // the waves' parts, added in their order
+            __syncthreads();
+            #pragma unroll
+            for (int i = 0; i < NV; ++i)
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    lds[(threadIdx.x >> 6) * NV * 512 + (i * 8 + j) * 64 + t] =
+                        which ? db[i][j] : dw[i][j];
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.C; c += 256) {
+                const int at = ((c >> 9) * 8 + (c & 7)) * 64 + ((c >> 3) & 63);
+                part[c] = (lds[at] + lds[NV * 512 + at]) +
+                          (lds[2 * NV * 512 + at] + lds[3 * NV * 512 + at]);
+            }
+        } else {
+            #pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int col = (i * 64 * TW + t) * 8;
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (col + j < a.C) part[col + j] = which ? db[i][j] : dw[i][j];
+            }
+        }
+    }
 }
 
 template <typename T, typename W>
@@ -304,21 +445,24 @@ __global__ __launch_bounds__(256) void norm_part_long_kernel(NormBwd a) {
     part[a.C + c] = db;
 }
 
-// dw, db [C] = sum over G of part[g][2][C]; either may be null
+// dw, db [C] = sum over G of part[g][2][C]; either may be null.  64 columns
+// and 16 shares of the parts a workgroup: a load depends on none before it.
 template <typename W>
-__global__ __launch_bounds__(256) void norm_add_parts_kernel(
+__global__ __launch_bounds__(1024) void norm_add_parts_kernel(
     const float* __restrict__ part, W* __restrict__ dw, W* __restrict__ db,
     int G, int C) {
-    __shared__ float red[8][32];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), g0 = threadIdx.x >> 5;
+    __shared__ float red[16][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), g0 = threadIdx.x >> 6;
     float t = 0.0f;
-    if (c < 2 * C)
-        for (int g = g0; g < G; g += 8) t += part[(int64_t)g * 2 * C + c];
-    red[g0][threadIdx.x & 31] = t;
+    if (c < 2 * C) {
+        #pragma unroll 8
+        for (int g = g0; g < G; g += 16) t += part[(int64_t)g * 2 * C + c];
+    }
+    red[g0][threadIdx.x & 63] = t;
     __syncthreads();
     if (g0 == 0 && c < 2 * C) {
         #pragma unroll
-        for (int i = 1; i < 8; ++i) t += red[i][threadIdx.x];
+        for (int i = 1; i < 16; ++i) t += red[i][threadIdx.x];
         if (c < C) {
             if (dw) dw[c] = from_f<W>(t);
         } else if (db) {
@@ -339,11 +483,14 @@ bool aligned8(const void* p, int64_t ld, int size) {
     else if (wtype == 2) { using T = fp16_t; using W = fp16_t; __VA_ARGS__; } \
     else { using T = fp16_t; using W = float; __VA_ARGS__; }
 
-#define RIQN_NORM_NV(C, ...)                                   \
-    if (C <= 512) { constexpr int NV = 1; __VA_ARGS__; }       \
-    else if (C <= 1024) { constexpr int NV = 2; __VA_ARGS__; } \
-    else if (C <= 2048) { constexpr int NV = 4; __VA_ARGS__; } \
-    else { constexpr int NV = 8; __VA_ARGS__; }
+// Columns -> waves a row and registers: 512 NV columns a wave.
+#define RIQN_NORM_SHAPE(C, ...)                                                \
+    if (C <= 512) { constexpr int TW = 1, NV = 1; __VA_ARGS__; }               \
+    else if (C <= 1024) { constexpr int TW = 1, NV = 2; __VA_ARGS__; }         \
+    else if (C <= 2048) { constexpr int TW = 4, NV = 1; __VA_ARGS__; }         \
+    else { constexpr int TW = 4, NV = 2; __VA_ARGS__; }
+
+int teams_of(int C) { return C <= 1024 ? 4 : 1; }
 
 }  // namespace
 
@@ -363,18 +510,25 @@ int riqn_norm_fwd(const void* x, int type, int64_t ldx, const void* w,
             hipLaunchKernelGGL((norm_fwd_long_kernel<T, W>),
                                dim3(min(R, 1 << 16)), dim3(256), 0, st, a);
         } else {
-            const dim3 grid((R + 3) / 4);
-            RIQN_NORM_NV(C, {
+            const int rows = RB * teams_of(C);  // of a workgroup at a time
+            const dim3 grid(min((R + rows - 1) / rows, 2048));
+            RIQN_NORM_SHAPE(C, {
                 if (vec)
-                    hipLaunchKernelGGL((norm_fwd_kernel<T, W, NV, true>), grid,
-                                       dim3(256), 0, st, a);
+                    hipLaunchKernelGGL((norm_fwd_kernel<T, W, TW, NV, true>),
+                                       grid, dim3(256), 0, st, a);
                 else
-                    hipLaunchKernelGGL((norm_fwd_kernel<T, W, NV, false>),
+                    hipLaunchKernelGGL((norm_fwd_kernel<T, W, TW, NV, false>),
                                        grid, dim3(256), 0, st, a);
             })
         }
     })
     return (int)hipGetLastError();
+}
+
+// workgroups of the backward pass, each of which leaves a part
+int riqn_norm_groups(int R, int C) {
+    const int rows = C > 4096 ? 4 : RB * teams_of(C);
+    return min((R + rows - 1) / rows, 512);
 }
 
 // part: [groups][2][C] fp32 workspace, or null where neither dw nor db is
@@ -399,20 +553,19 @@ int riqn_norm_bwd(const void* dy, const void* x, int type, int64_t lddy,
                                    dim3(groups, (C + 255) / 256), dim3(256), 0,
                                    st, a);
         } else {
-            const uint32_t bytes = part ? 2 * C * sizeof(float) : 0;
-            RIQN_NORM_NV(C, {
+            RIQN_NORM_SHAPE(C, {
                 if (vec)
-                    hipLaunchKernelGGL((norm_bwd_kernel<T, W, NV, true>),
-                                       dim3(groups), dim3(256), bytes, st, a);
+                    hipLaunchKernelGGL((norm_bwd_kernel<T, W, TW, NV, true>),
+                                       dim3(groups), dim3(256), 0, st, a);
                 else
-                    hipLaunchKernelGGL((norm_bwd_kernel<T, W, NV, false>),
-                                       dim3(groups), dim3(256), bytes, st, a);
+                    hipLaunchKernelGGL((norm_bwd_kernel<T, W, TW, NV, false>),
+                                       dim3(groups), dim3(256), 0, st, a);
             })
         }
         if (part)
             hipLaunchKernelGGL((norm_add_parts_kernel<W>),
-                               dim3((2 * C + 31) / 32), dim3(256), 0, st, part,
-                               (W*)dw, (W*)db, groups, C);
+                               dim3((2 * C + 63) / 64), dim3(1024), 0, st,
+                               part, (W*)dw, (W*)db, groups, C);
     })
     return (int)hipGetLastError();
 }

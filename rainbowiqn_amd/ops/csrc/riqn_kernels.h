@@ -179,6 +179,7 @@ int riqn_fp8_wgrad(const uint8_t* g, const uint8_t* gs, const uint8_t* x,
 int riqn_norm_fwd(const void* x, int type, int64_t ldx, const void* w,
                   const void* b, int wtype, void* y, float* mean, float* rstd,
                   int R, int C, float eps, void* stream);
+int riqn_norm_groups(int R, int C);
 int riqn_norm_bwd(const void* dy, const void* x, int type, int64_t lddy,
                   int64_t ldx, const void* w, int wtype, const float* mean,
                   const float* rstd, void* dx, void* dw, void* db, float* part,
