@@ -320,9 +320,9 @@ LinearGrads linear_bwd(const Tensor& dy, const LinearSaved& s, int64_t K,
         gemm(g, wt, N, c10::nullopt, false, o.dx, nullptr);
     }
     if (dw_type) {
-        // a share of the rows for each workgroup of a tile: enough for two
-        // workgroups a CU, and at least 256 rows each
-        const int64_t tiles = blocks_of(N) * blocks_of(K);
+        // shares of the rows for each tile of 256 x 128: as many as two
+        // workgroups a CU make one round of, with at least 256 rows each
+        const int64_t tiles = (blocks_of(N) + 1) / 2 * blocks_of(K);
         const int shares = (int)std::max<int64_t>(
             1, std::min<int64_t>(std::min<int64_t>(512 / tiles, M / 256), 64));
         Tensor part;

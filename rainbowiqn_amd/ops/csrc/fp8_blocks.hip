@@ -178,20 +178,23 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(
     }
 }
 
-// out[c] = sum over G rows of part[g][c]
+// out[c] = sum over G rows of part[g][c]; 64 columns and 16 shares of the rows
+// a workgroup, so that no load waits for another
 template <typename T>
-__global__ __launch_bounds__(256) void column_sum_kernel(
+__global__ __launch_bounds__(1024) void column_sum_kernel(
     const float* __restrict__ part, T* __restrict__ out, int G, int C) {
-    __shared__ float red[8][32];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), g0 = threadIdx.x >> 5;
+    __shared__ float red[16][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), g0 = threadIdx.x >> 6;
     float t = 0.0f;
-    if (c < C)
-        for (int g = g0; g < G; g += 8) t += part[(int64_t)g * C + c];
-    red[g0][threadIdx.x & 31] = t;
+    if (c < C) {
+        #pragma unroll 8
+        for (int g = g0; g < G; g += 16) t += part[(int64_t)g * C + c];
+    }
+    red[g0][threadIdx.x & 63] = t;
     __syncthreads();
     if (g0 == 0 && c < C) {
         #pragma unroll
-        for (int i = 1; i < 8; ++i) t += red[i][threadIdx.x];
+        for (int i = 1; i < 16; ++i) t += red[i][threadIdx.x];
         out[c] = from_f<T>(t);
     }
 }
@@ -256,17 +259,33 @@ __global__ __launch_bounds__(256) void quant_tiles_kernel(
     }
     if (!qt) return;
     __syncthreads();
-    // row c of the transposed block: 128 bytes, 8 per lane of 16
+    // 8 rows x 4 columns a turn, transposed by byte permutes; 16 lanes write
+    // the 128 bytes of one row of the transposed block
     #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = i * 16 + rr;
-        if (bc * 128 + c < C) {
-            uint32_t w[2] = {0, 0};
-            #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                w[j >> 2] |= (uint32_t)tile[l15 * 8 + j][c] << (8 * (j & 3));
-            *(i32x2*)(qt + (int64_t)(bc * 128 + c) * (nbt * 128) + br * 128 +
-                      l15 * 8) = i32x2{(int)w[0], (int)w[1]};
+    for (int i = 0; i < 2; ++i) {
+        const int n8 = t & 15, c4 = i * 16 + (t >> 4);
+        uint32_t d[8], o[4][2];
+        #pragma unroll
+        for (int r = 0; r < 8; ++r)
+            d[r] = *(const uint32_t*)&tile[n8 * 8 + r][c4 * 4];
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t* e = d + 4 * h;
+            const uint32_t a = __builtin_amdgcn_perm(e[1], e[0], 0x05010400);
+            const uint32_t b = __builtin_amdgcn_perm(e[1], e[0], 0x07030602);
+            const uint32_t u = __builtin_amdgcn_perm(e[3], e[2], 0x05010400);
+            const uint32_t v = __builtin_amdgcn_perm(e[3], e[2], 0x07030602);
+            o[0][h] = __builtin_amdgcn_perm(u, a, 0x05040100);
+            o[1][h] = __builtin_amdgcn_perm(u, a, 0x07060302);
+            o[2][h] = __builtin_amdgcn_perm(v, b, 0x05040100);
+            o[3][h] = __builtin_amdgcn_perm(v, b, 0x07060302);
+        }
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int c = bc * 128 + c4 * 4 + r;
+            if (c < C)
+                *(i32x2*)(qt + (int64_t)c * (nbt * 128) + br * 128 + n8 * 8) =
+                    i32x2{(int)o[r][0], (int)o[r][1]};
         }
     }
 }
@@ -704,28 +723,36 @@ void launch_tiles(const Gemm& g, hipStream_t st) {
 // is rounded before the fp32 sums.  LDS keeps rows of m; ds_read_b64_tr_b16 hands each lane 4
 // rows of one column, the operand layout of a product that sums over rows.
 //
-// A tile is 128 x 128, one block of each operand, 64 rows a step, 4 waves of
-// 64 x 64.  The 256-byte LDS rows are stored in 32-byte pieces at piece ^
-// (row & 7), so that the 16 rows of a transposed read fall on all banks.
+// A tile is 256 x 128, 32 rows a step, 4 waves of 128 x 64; two LDS buffers
+// of 24 KB leave room for a second workgroup on the CU, whose waves multiply
+// while this one's wait at a barrier.  Loads run 3 steps ahead in registers:
+// a step is shorter than the way to memory.  The rows of LDS are stored in
+// 32-byte pieces at piece ^ (row & 7), so that the 16 rows of a transposed
+// read fall on all banks; within 64 columns of X, column 16 a + 4 j + b lies
+// at 16 j + 4 a + b, so that a lane ends up with 16 neighbours of one row of
+// dW.
+//
 // blockIdx.y takes a share of the rows; with more than one share each writes
 // fp32 partials [share][N][K], added in a fixed order by add_shares_kernel.
 // ---------------------------------------------------------------------------
 struct Wgrad {
     const uint8_t *g, *gs, *x, *xs;  // [M, 128 nbn], [M, Sn], [M, 128 nbk], ...
     void* dw;                        // [N, K] of T, or fp32 [shares][N][K]
-    int M, N, K, nbn, Sn, nbk, Sk, rows;  // rows of a share: multiple of 64
+    int M, N, K, nbn, Sn, nbk, Sk, rows;  // rows of a share: multiple of 32
 };
 
-// the 16 rows m = l4 * 4 ... of 16 columns from c: bf16 [64][128] swizzled
-DEV bf16x8 tr_frag(const uint16_t* tile, int m, int c, int lane) {
+// rows m ... m + 31 of the 16 columns from c of a tile of W columns; lane
+// group l4 gets rows 4 l4 ... and 16 + 4 l4 ..., in both operands alike
+template <int W>
+DEV bf16x8 tr_frag(const uint16_t* tile, int c, int lane) {
     const int l15 = lane & 15, l4 = lane >> 4;
     bf16x8 f;
     #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int row = m + h * 16 + l4 * 4 + (l15 >> 2);
+        const int row = h * 16 + l4 * 4 + (l15 >> 2);
         const int piece = (c >> 4) ^ (row & 7);
         auto* p = (__attribute__((address_space(3))) s16x4*)(
-            tile + row * 128 + piece * 16 + (l15 & 3) * 4);
+            tile + row * W + piece * 16 + (l15 & 3) * 4);
         const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
         const bf16x4 b = __builtin_bit_cast(bf16x4, v);
         #pragma unroll
@@ -734,81 +761,114 @@ DEV bf16x8 tr_frag(const uint16_t* tile, int m, int c, int lane) {
     return f;
 }
 
-DEV void expand_store(uint16_t* tile, int row, int piece, i32x4 w, int sbyte) {
-    // 16 values = one 32-byte piece of the row
-    i32x4* p = (i32x4*)(tile + row * 128 + (piece ^ (row & 7)) * 16);
-    p[0] = __builtin_bit_cast(i32x4, expand8(w[0], w[1], sbyte));
-    p[1] = __builtin_bit_cast(i32x4, expand8(w[2], w[3], sbyte));
-}
-
 template <typename T>
-__global__ __launch_bounds__(256) void wgrad_kernel(Wgrad w) {
-    __shared__ __align__(16) uint16_t gt[64 * 128], xt[64 * 128];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+__global__ __launch_bounds__(256, 2) void wgrad_kernel(Wgrad w) {
+    __shared__ __align__(16) uint16_t gt[2][32 * 256], xt[2][32 * 128];
+    const int t = threadIdx.x, lane = t & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int l15 = lane & 15, l4 = lane >> 4;
-    const int bn = blockIdx.x / w.nbk, bk = blockIdx.x % w.nbk;
-    const int wn = (wave >> 1) * 64, wk = (wave & 1) * 64;
+    const int bn = blockIdx.x / w.nbk * 2, bk = blockIdx.x % w.nbk;
+    const int wn = (wave >> 1) * 128, wk = (wave & 1) * 64;
     const int64_t ldg = (int64_t)w.nbn * 128, ldx = (int64_t)w.nbk * 128;
     const int lo = blockIdx.y * w.rows, hi = min(lo + w.rows, w.M);
-    f32x4 acc[4][4];
+    const int steps = (hi - lo + 31) >> 5;  // <= 0 where nothing is left
+
+    // 16 bytes each: rows t / 16 and 16 + t / 16 of G, row t / 8 of X
+    struct Held { i32x4 v[3]; int e[3]; };
+    auto load = [&](Held& h, int step) {
+        #pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const int row = i < 2 ? i * 16 + (t >> 4) : t >> 3;
+            const int piece = i < 2 ? t & 15 : t & 7;
+            const int64_t m = lo + (int64_t)step * 32 + row;
+            const int blk = i < 2 ? bn + (piece >> 3) : bk;
+            h.v[i] = i32x4{0, 0, 0, 0};
+            h.e[i] = 127;
+            if (m < hi && (i == 2 || blk < w.nbn)) {
+                h.v[i] = i < 2 ? *(const i32x4*)(w.g + m * ldg + bn * 128 + piece * 16)
+                               : *(const i32x4*)(w.x + m * ldx + bk * 128 + piece * 16);
+                h.e[i] = i < 2 ? w.gs[m * w.Sn + blk] : w.xs[m * w.Sk + blk];
+            }
+        }
+    };
+    auto store = [&](const Held& h, int buf) {
+        #pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const bf16x8 a = expand8(h.v[i][0], h.v[i][1], h.e[i]);
+            const bf16x8 b = expand8(h.v[i][2], h.v[i][3], h.e[i]);
+            if (i < 2) {
+                const int row = i * 16 + (t >> 4), piece = t & 15;
+                bf16x8* p = (bf16x8*)&gt[buf][row * 256 + (piece ^ (row & 7)) * 16];
+                p[0] = a;
+                p[1] = b;
+            } else {
+                const int row = t >> 3, piece = t & 7;
+                const i32x4 u = __builtin_bit_cast(i32x4, a);
+                const i32x4 v = __builtin_bit_cast(i32x4, b);
+                const int part[4][2] = {{u[0], u[1]}, {u[2], u[3]},
+                                        {v[0], v[1]}, {v[2], v[3]}};
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int to = (piece >> 2) * 4 + j;  // 32-byte piece
+                    *(i32x2*)&xt[buf][row * 128 + (to ^ (row & 7)) * 16 +
+                                      (piece & 3) * 4] =
+                        i32x2{part[j][0], part[j][1]};
+                }
+            }
+        }
+    };
+    f32x4 acc[8][4];
     #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i)
         #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    for (int m0 = lo; m0 < hi; m0 += 64) {
-        // 64 rows x 8 pieces of 16 bytes: 2 per thread and operand
+    Held h0, h1;  // even and odd steps
+    load(h0, 0);
+    load(h1, 1);
+    store(h0, 0);
+    load(h0, 2);
+    __syncthreads();
+    auto turn = [&](Held& next, int step, int buf) {
+        // the other buffer: all waves are past reading it
+        if (step + 1 < steps) store(next, buf ^ 1);
+        if (step + 3 < steps) load(next, step + 3);
+        bf16x8 fx[4];
         #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = i * 32 + (t >> 3), piece = t & 7;
-            const int64_t m = m0 + row;
-            i32x4 gv = {0, 0, 0, 0}, xv = {0, 0, 0, 0};
-            int ge = 127, xe = 127;
-            if (m < hi) {
-                gv = *(const i32x4*)(w.g + m * ldg + bn * 128 + piece * 16);
-                xv = *(const i32x4*)(w.x + m * ldx + bk * 128 + piece * 16);
-                ge = w.gs[m * w.Sn + bn];
-                xe = w.xs[m * w.Sk + bk];
-            }
-            expand_store(gt, row, piece, gv, ge);
-            expand_store(xt, row, piece, xv, xe);
+        for (int j = 0; j < 4; ++j) fx[j] = tr_frag<128>(xt[buf], wk + j * 16, lane);
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bf16x8 fg = tr_frag<256>(gt[buf], wn + i * 16, lane);
+            // rows of the MFMA's result are k, columns n
+            #pragma unroll
+            for (int j = 0; j < 4; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    fx[j], fg, acc[i][j], 0, 0, 0);
         }
         __syncthreads();
-        #pragma unroll
-        for (int ms = 0; ms < 64; ms += 32) {
-            bf16x8 fg[4], fx[4];
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                fg[i] = tr_frag(gt, ms, wn + i * 16, lane);
-                fx[i] = tr_frag(xt, ms, wk + i * 16, lane);
-            }
-            // rows of the result are k, so a lane holds 4 neighbours of a row
-            #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        fx[j], fg[i], acc[i][j], 0, 0, 0);
-        }
-        __syncthreads();
+    };
+    for (int step = 0; step < steps; step += 2) {
+        turn(h1, step, 0);
+        if (step + 1 < steps) turn(h0, step + 1, 1);
     }
+    const int k = bk * 128 + wk + l4 * 16;
+    if (k >= w.K) return;
+    const bool whole = k + 16 <= w.K && (w.K * sizeof(T) & 15) == 0;
     #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
         const int n = bn * 128 + wn + i * 16 + l15;
         if (n >= w.N) continue;
+        struct alignas(16) Pack { T t[16]; } p;
         #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = bk * 128 + wk + j * 16 + l4 * 4;
-            T* out = (T*)w.dw + ((int64_t)blockIdx.y * w.N + n) * w.K + k;
-            struct alignas(4 * sizeof(T)) Pack { T t[4]; } p;
+        for (int j = 0; j < 4; ++j)
             #pragma unroll
-            for (int e = 0; e < 4; ++e) p.t[e] = from_f<T>(acc[i][j][e]);
-            if ((w.K & 3) == 0) {
-                if (k < w.K) *(Pack*)out = p;
-            } else {
-                #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (k + e < w.K) out[e] = p.t[e];
-            }
+            for (int e = 0; e < 4; ++e) p.t[j * 4 + e] = from_f<T>(acc[i][j][e]);
+        T* out = (T*)w.dw + ((int64_t)blockIdx.y * w.N + n) * w.K + k;
+        if (whole) {
+            *(Pack*)out = p;
+        } else {
+            #pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (k + e < w.K) out[e] = p.t[e];
         }
     }
 }
@@ -869,7 +929,7 @@ int riqn_fp8_quant_rows(const void* x, int type, int64_t ldx,
 int riqn_column_sum(const float* part, void* out, int type, int G, int C,
                     void* stream) {
     RIQN_TYPE(type, T, hipLaunchKernelGGL(
-        column_sum_kernel<T>, dim3((C + 31) / 32), dim3(256), 0,
+        column_sum_kernel<T>, dim3((C + 63) / 64), dim3(1024), 0,
         (hipStream_t)stream, part, (T*)out, G, C))
     return (int)hipGetLastError();
 }
@@ -946,11 +1006,11 @@ int riqn_fp8_wgrad(const uint8_t* g, const uint8_t* gs, const uint8_t* x,
                    const uint8_t* xs, void* dw, int type, float* part,
                    int shares, int M, int N, int K, void* stream) {
     const int nbn = (N + 127) >> 7, nbk = (K + 127) >> 7;
-    const int rows = ((M + shares - 1) / shares + 63) & ~63;
+    const int rows = ((M + shares - 1) / shares + 31) & ~31;
     Wgrad w{g, gs, x, xs, shares > 1 ? (void*)part : dw, M, N, K, nbn,
             (nbn + 3) & ~3, nbk, (nbk + 3) & ~3, rows};
     hipStream_t st = (hipStream_t)stream;
-    dim3 grid(nbn * nbk, shares);
+    dim3 grid((nbn + 1) / 2 * nbk, shares);
     RIQN_TYPE(shares > 1 ? 0 : type, T, hipLaunchKernelGGL(
         wgrad_kernel<T>, grid, dim3(256), 0, st, w))
     if (shares > 1) {
