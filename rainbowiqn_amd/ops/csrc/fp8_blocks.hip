@@ -725,34 +725,50 @@ void launch_tiles(const Gemm& g, hipStream_t st) {
 //
 // A tile is 256 x 128, 32 rows a step, 4 waves of 128 x 64; two LDS buffers
 // of 24 KB leave room for a second workgroup on the CU, whose waves multiply
-// while this one's wait at a barrier.  Loads run 3 steps ahead in registers:
-// a step is shorter than the way to memory.  The rows of LDS are stored in
-// 32-byte pieces at piece ^ (row & 7), so that the 16 rows of a transposed
-// read fall on all banks; within 64 columns of X, column 16 a + 4 j + b lies
-// at 16 j + 4 a + b, so that a lane ends up with 16 neighbours of one row of
-// dW.
+// while this one's wait at a barrier.  Loads run 3 steps ahead in registers: a
+// step is shorter than the way to memory.  They go by a buffer that ends with
+// the last row, behind which they give zeros: none is conditional, so the
+// compiler waits for those of one step only.
 //
-// blockIdx.y takes a share of the rows; with more than one share each writes
-// fp32 partials [share][N][K], added in a fixed order by add_shares_kernel.
+// LDS keeps rows of m in an order that spreads what 16 rows of a transposed
+// read, or 16 lanes of a write, touch over all banks.  Within 64 columns of X,
+// column 16 a + 4 j + b lies at 16 j + 4 a + b, so that a lane ends up with 16
+// neighbours of one row of dW.
+//
+// A workgroup takes one tile and one share of the rows; with more than one
+// share each writes fp32 partials [share][N][K], added in a fixed order by
+// add_shares_kernel.
 // ---------------------------------------------------------------------------
 struct Wgrad {
     const uint8_t *g, *gs, *x, *xs;  // [M, 128 nbn], [M, Sn], [M, 128 nbk], ...
     void* dw;                        // [N, K] of T, or fp32 [shares][N][K]
-    int M, N, K, nbn, Sn, nbk, Sk, rows;  // rows of a share: multiple of 32
+    int M, N, K, nbn, Sn, nbk, Sk;
+    int shares, rows;  // rows of a share: multiple of 64
 };
 
-// rows m ... m + 31 of the 16 columns from c of a tile of W columns; lane
-// group l4 gets rows 4 l4 ... and 16 + 4 l4 ..., in both operands alike
-template <int W>
+// Where 8 bytes (4 columns from c) of a row lie.  G: rows of 256 columns, the
+// two 16-byte halves of 16 columns 256 bytes apart; X: rows of 128 columns, 16
+// columns together.
+DEV int at_g(int row, int c) {
+    const int half = (c >> 3) & 1;
+    return row * 256 + half * 128 + ((c >> 4) ^ (8 * half) ^ (row & 7)) * 8 +
+           (c & 7);
+}
+DEV int at_x(int row, int c) {
+    return row * 128 + ((c >> 4) ^ (row & 7)) * 16 + (c & 15);
+}
+
+// the 32 rows of the 16 columns from c; lane group l4 gets rows 4 l4 ... and
+// 16 + 4 l4 ..., in both operands alike
+template <bool G>
 DEV bf16x8 tr_frag(const uint16_t* tile, int c, int lane) {
     const int l15 = lane & 15, l4 = lane >> 4;
     bf16x8 f;
     #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int row = h * 16 + l4 * 4 + (l15 >> 2);
-        const int piece = (c >> 4) ^ (row & 7);
+        const int row = h * 16 + l4 * 4 + (l15 >> 2), cc = c + (l15 & 3) * 4;
         auto* p = (__attribute__((address_space(3))) s16x4*)(
-            tile + row * W + piece * 16 + (l15 & 3) * 4);
+            tile + (G ? at_g(row, cc) : at_x(row, cc)));
         const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
         const bf16x4 b = __builtin_bit_cast(bf16x4, v);
         #pragma unroll
@@ -763,58 +779,65 @@ DEV bf16x8 tr_frag(const uint16_t* tile, int c, int lane) {
 
 template <typename T>
 __global__ __launch_bounds__(256, 2) void wgrad_kernel(Wgrad w) {
+#ifdef __HIP_DEVICE_COMPILE__
     __shared__ __align__(16) uint16_t gt[2][32 * 256], xt[2][32 * 128];
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int l15 = lane & 15, l4 = lane >> 4;
-    const int bn = blockIdx.x / w.nbk * 2, bk = blockIdx.x % w.nbk;
+    // each XCD takes one run of tiles of the same share, which walk over the
+    // same rows side by side: its L2 fetches them once.  Dealt out one by one
+    // instead, every XCD fetches everything, and memory sets the pace.
+    const int xcd = blockIdx.x & 7, q = gridDim.x >> 3, rem = gridDim.x & 7;
+    const int at = xcd * q + min(xcd, rem) + (blockIdx.x >> 3);
+    const int tiles = gridDim.x / w.shares;
+    const int share = at / tiles, tile = at - share * tiles;
+    const int bn = tile / w.nbk * 2, bk = tile % w.nbk;
     const int wn = (wave >> 1) * 128, wk = (wave & 1) * 64;
     const int64_t ldg = (int64_t)w.nbn * 128, ldx = (int64_t)w.nbk * 128;
-    const int lo = blockIdx.y * w.rows, hi = min(lo + w.rows, w.M);
-    const int steps = (hi - lo + 31) >> 5;  // <= 0 where nothing is left
+    const int lo = share * w.rows, hi = min(lo + w.rows, w.M);
+    // an even number of steps; the last may lie behind row M, among zeros
+    const int steps = ((hi - lo + 63) >> 6) * 2;  // <= 0: nothing is left
 
-    // 16 bytes each: rows t / 16 and 16 + t / 16 of G, row t / 8 of X
+    // 16 bytes each: rows t / 16 and 16 + t / 16 of G, row t / 8 of X.  A
+    // second block of G that is not there is read as the first.
+    const int pg = t & 15, px = t & 7, rg = t >> 4, rx = t >> 3;
+    const bool there = bn + (pg >> 3) < w.nbn;
+    const int og = rg * (int)ldg + bn * 128 + (there ? pg : pg & 7) * 16;
+    const int os = rg * w.Sn + bn + (there ? pg >> 3 : 0);
+    const int ox = rx * (int)ldx + bk * 128 + px * 16, ot = rx * w.Sk + bk;
     struct Held { i32x4 v[3]; int e[3]; };
     auto load = [&](Held& h, int step) {
+        const int64_t m = lo + (int64_t)step * 32;
+        const int64_t left = max((int64_t)0, w.M - m);
+        const auto bg = buffer_of(w.g + m * ldg, left * ldg);
+        const auto bs = buffer_of(w.gs + m * w.Sn, left * w.Sn);
+        const auto bx = buffer_of(w.x + m * ldx, left * ldx);
+        const auto bt = buffer_of(w.xs + m * w.Sk, left * w.Sk);
         #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            const int row = i < 2 ? i * 16 + (t >> 4) : t >> 3;
-            const int piece = i < 2 ? t & 15 : t & 7;
-            const int64_t m = lo + (int64_t)step * 32 + row;
-            const int blk = i < 2 ? bn + (piece >> 3) : bk;
-            h.v[i] = i32x4{0, 0, 0, 0};
-            h.e[i] = 127;
-            if (m < hi && (i == 2 || blk < w.nbn)) {
-                h.v[i] = i < 2 ? *(const i32x4*)(w.g + m * ldg + bn * 128 + piece * 16)
-                               : *(const i32x4*)(w.x + m * ldx + bk * 128 + piece * 16);
-                h.e[i] = i < 2 ? w.gs[m * w.Sn + blk] : w.xs[m * w.Sk + blk];
-            }
+        for (int i = 0; i < 2; ++i) {
+            h.v[i] = __builtin_amdgcn_raw_buffer_load_b128(
+                bg, og, i * 16 * (int)ldg, 0);
+            h.e[i] = __builtin_amdgcn_raw_buffer_load_b8(bs, os, i * 16 * w.Sn, 0);
         }
+        h.v[2] = __builtin_amdgcn_raw_buffer_load_b128(bx, ox, 0, 0);
+        h.e[2] = __builtin_amdgcn_raw_buffer_load_b8(bt, ot, 0, 0);
     };
     auto store = [&](const Held& h, int buf) {
         #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            const bf16x8 a = expand8(h.v[i][0], h.v[i][1], h.e[i]);
-            const bf16x8 b = expand8(h.v[i][2], h.v[i][3], h.e[i]);
-            if (i < 2) {
-                const int row = i * 16 + (t >> 4), piece = t & 15;
-                bf16x8* p = (bf16x8*)&gt[buf][row * 256 + (piece ^ (row & 7)) * 16];
-                p[0] = a;
-                p[1] = b;
-            } else {
-                const int row = t >> 3, piece = t & 7;
-                const i32x4 u = __builtin_bit_cast(i32x4, a);
-                const i32x4 v = __builtin_bit_cast(i32x4, b);
-                const int part[4][2] = {{u[0], u[1]}, {u[2], u[3]},
-                                        {v[0], v[1]}, {v[2], v[3]}};
-                #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int to = (piece >> 2) * 4 + j;  // 32-byte piece
-                    *(i32x2*)&xt[buf][row * 128 + (to ^ (row & 7)) * 16 +
-                                      (piece & 3) * 4] =
-                        i32x2{part[j][0], part[j][1]};
-                }
-            }
+        for (int i = 0; i < 2; ++i) {
+            const int row = i * 16 + rg;
+            *(bf16x8*)&gt[buf][at_g(row, pg * 16)] =
+                expand8(h.v[i][0], h.v[i][1], h.e[i]);
+            *(bf16x8*)&gt[buf][at_g(row, pg * 16 + 8)] =
+                expand8(h.v[i][2], h.v[i][3], h.e[i]);
+        }
+        #pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+            const i32x4 u = __builtin_bit_cast(
+                i32x4, expand8(h.v[2][j], h.v[2][j + 1], h.e[2]));
+            const int c = (px >> 2) * 64 + (px & 3) * 4;
+            *(i32x2*)&xt[buf][at_x(rx, c + j * 16)] = i32x2{u[0], u[1]};
+            *(i32x2*)&xt[buf][at_x(rx, c + j * 16 + 16)] = i32x2{u[2], u[3]};
         }
     };
     f32x4 acc[8][4];
@@ -829,26 +852,31 @@ __global__ __launch_bounds__(256, 2) void wgrad_kernel(Wgrad w) {
     load(h0, 2);
     __syncthreads();
     auto turn = [&](Held& next, int step, int buf) {
-        // the other buffer: all waves are past reading it
-        if (step + 1 < steps) store(next, buf ^ 1);
-        if (step + 3 < steps) load(next, step + 3);
-        bf16x8 fx[4];
+        store(next, buf ^ 1);  // all waves are past reading it
+        load(next, step + 3);
+        __builtin_amdgcn_sched_barrier(0);  // the loads are under way
+        // all reads first: the way to LDS is waited for once
+        bf16x8 fx[4], fg[8];
         #pragma unroll
-        for (int j = 0; j < 4; ++j) fx[j] = tr_frag<128>(xt[buf], wk + j * 16, lane);
+        for (int j = 0; j < 4; ++j)
+            fx[j] = tr_frag<false>(xt[buf], wk + j * 16, lane);
         #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bf16x8 fg = tr_frag<256>(gt[buf], wn + i * 16, lane);
-            // rows of the MFMA's result are k, columns n
+        for (int i = 0; i < 8; ++i)
+            fg[i] = tr_frag<true>(gt[buf], wn + i * 16, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        // rows of the MFMA's result are k, columns n
+        #pragma unroll
+        for (int i = 0; i < 8; ++i)
             #pragma unroll
             for (int j = 0; j < 4; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    fx[j], fg, acc[i][j], 0, 0, 0);
-        }
+                    fx[j], fg[i], acc[i][j], 0, 0, 0);
         __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
     };
     for (int step = 0; step < steps; step += 2) {
         turn(h1, step, 0);
-        if (step + 1 < steps) turn(h0, step + 1, 1);
+        turn(h0, step + 1, 1);
     }
     const int k = bk * 128 + wk + l4 * 16;
     if (k >= w.K) return;
@@ -862,7 +890,7 @@ __global__ __launch_bounds__(256, 2) void wgrad_kernel(Wgrad w) {
         for (int j = 0; j < 4; ++j)
             #pragma unroll
             for (int e = 0; e < 4; ++e) p.t[j * 4 + e] = from_f<T>(acc[i][j][e]);
-        T* out = (T*)w.dw + ((int64_t)blockIdx.y * w.N + n) * w.K + k;
+        T* out = (T*)w.dw + ((int64_t)share * w.N + n) * w.K + k;
         if (whole) {
             *(Pack*)out = p;
         } else {
@@ -871,6 +899,7 @@ __global__ __launch_bounds__(256, 2) void wgrad_kernel(Wgrad w) {
                 if (k + e < w.K) out[e] = p.t[e];
         }
     }
+#endif
 }
 
 template <typename T>
@@ -1006,11 +1035,11 @@ int riqn_fp8_wgrad(const uint8_t* g, const uint8_t* gs, const uint8_t* x,
                    const uint8_t* xs, void* dw, int type, float* part,
                    int shares, int M, int N, int K, void* stream) {
     const int nbn = (N + 127) >> 7, nbk = (K + 127) >> 7;
-    const int rows = ((M + shares - 1) / shares + 31) & ~31;
+    const int rows = ((M + shares - 1) / shares + 63) & ~63;
     Wgrad w{g, gs, x, xs, shares > 1 ? (void*)part : dw, M, N, K, nbn,
-            (nbn + 3) & ~3, nbk, (nbk + 3) & ~3, rows};
+            (nbn + 3) & ~3, nbk, (nbk + 3) & ~3, shares, rows};
     hipStream_t st = (hipStream_t)stream;
-    dim3 grid((nbn + 1) / 2 * nbk, shares);
+    dim3 grid((nbn + 1) / 2 * nbk * shares);
     RIQN_TYPE(shares > 1 ? 0 : type, T, hipLaunchKernelGGL(
         wgrad_kernel<T>, grid, dim3(256), 0, st, w))
     if (shares > 1) {
