@@ -472,7 +472,7 @@ __global__ __launch_bounds__(512) void gemm_direct_kernel(Gemm g) {
 
 // ---------------------------------------------------------------------------
 // Larger results.  A workgroup of WM x WN waves, each with 16 MI rows of C and
-// 64 columns, walks over K in steps of 128 with two LDS buffers: while one is
+// 16 NJ columns, walks over K in steps of 128 with two LDS buffers: while one is
 // multiplied the next is on its way into the other, straight from memory
 // (global_load_lds, 16 bytes a lane).  The walk goes on over the workgroup's
 // next tile without a pause: its first step is under way during the epilogue.
@@ -498,16 +498,19 @@ DEV __amdgpu_buffer_rsrc_t buffer_of(const uint8_t* p, int64_t bytes) {
         (void*)p, 0, (int)min(bytes, (int64_t)0xffffffffu), 0x00027000);
 }
 
-template <int WM, int WN, int MI, bool EXACT, typename T>
+template <int WM, int WN, int MI, int NJ, bool EXACT, typename T>
 __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host needs its launch alone
-    constexpr int TM = WM * MI * 16, TN = WN * 64, WAVES = WM * WN;
+    constexpr int TM = WM * MI * 16, TN = WN * NJ * 16, WAVES = WM * WN;
     constexpr int BUF = (TM + TN) * 128;
-    extern __shared__ __align__(16) uint8_t lds[];  // [2][BUF]
+    // [2][BUF] tiles, [2][TM + TN] dwords of scales
+    extern __shared__ __align__(16) uint8_t lds[];
+    uint32_t* const lds_s = (uint32_t*)(lds + 2 * BUF);
+    static_assert(TM + TN == 64 * WAVES, "a scale a lane");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l15 = lane & 15, l4 = lane >> 4;
-    const int wm = (wave / WN) * MI * 16, wn = (wave % WN) * 64;
+    const int wm = (wave / WN) * MI * 16, wn = (wave % WN) * NJ * 16;
     const int nt = (g.N + TN - 1) / TN, mt = (g.M + TM - 1) / TM;
     const int64_t ld = (int64_t)g.nb * 128;
     // each XCD (workgroups are dealt to 8 in turn) takes one run of tiles,
@@ -524,8 +527,12 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
     // rows: lane -> row lane / 8, stored piece lane % 8; rows behind the last
     // one are read as the last.
     constexpr int LA = TM / 8 / WAVES, LB = TN / 8 / WAVES;
-    __amdgpu_buffer_rsrc_t buf_a, buf_b;
-    uint32_t off[LA + LB];
+    __amdgpu_buffer_rsrc_t buf_a, buf_b, buf_s;
+    uint32_t off[LA + LB], off_s;
+    // B's row at place r of a tile, see above
+    auto place = [](int r) {
+        return (r & ~63) + ((r & 15) >> 2) * 16 + ((r >> 4) & 3) * 4 + (r & 3);
+    };
     auto enter = [&](int tile) {
         const int m0 = (tile / nt) * TM, n0 = (tile % nt) * TN;
         buf_a = buffer_of(g.a + m0 * ld, (g.M - m0) * ld);
@@ -535,16 +542,37 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
             const int inst = (i < LA ? i : i - LA) * WAVES + wave;
             const int r = inst * 8 + (lane >> 3);
             const int from = i < LA ? min(r, g.M - 1 - m0)
-                                    : min((r & ~63) + ((r & 15) >> 2) * 16 +
-                                              ((r >> 4) & 3) * 4 + (r & 3),
-                                          g.N - 1 - n0);
+                                    : min(place(r), g.N - 1 - n0);
             off[i] = (uint32_t)from * (uint32_t)ld +
                      ((lane & 7) ^ ((r >> 1) & 7)) * 16;
         }
+        // scales: a wave takes those of 64 rows, A's or B's
+        const int r = wave * 64 + lane;
+        if (wave * 64 < TM) {
+            const int r0 = m0 >> g.ash;
+            buf_s = buffer_of(g.as + (int64_t)r0 * g.S,
+                              (((g.M - 1) >> g.ash) + 1 - r0) * (int64_t)g.S);
+            off_s = ((min(m0 + r, g.M - 1) >> g.ash) - r0) * g.S;
+        } else {
+            const int r0 = n0 >> g.bsh;
+            buf_s = buffer_of(g.bs + (int64_t)r0 * g.S,
+                              (((g.N - 1) >> g.bsh) + 1 - r0) * (int64_t)g.S);
+            off_s = ((min(n0 + place(r - TM), g.N - 1) >> g.bsh) - r0) * g.S;
+        }
     };
-    auto stage = [&](int buf, int kb) {
+    int sbuf = 1;  // which scales are in use
+    // loads [from, to) of a wave's share of a step
+    auto stage = [&](int buf, int kb, int from, int to) {
+        // the scales of 4 steps are a dword a row
+        if (from == 0 && (kb & 3) == 0)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                buf_s,
+                (__attribute__((address_space(3))) void*)(
+                    lds_s + (sbuf ^ 1) * (TM + TN) + wave * 64),
+                4, off_s, kb, 0, 0);
         #pragma unroll
         for (int i = 0; i < LA + LB; ++i) {
+            if (i < from || i >= to) continue;
             const int inst = (i < LA ? i : i - LA) * WAVES + wave;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 i < LA ? buf_a : buf_b,
@@ -554,166 +582,168 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
         }
     };
     enter(tile);
-    stage(0, 0);
+    stage(0, 0, 0, LA + LB);
     int buf = 0;
     for (; tile < end; tile += stride) {
         const int m0 = (tile / nt) * TM + wm, n0 = (tile % nt) * TN + wn;
-        f32x4 acc[MI][4];
+        f32x4 acc[MI][NJ];
         #pragma unroll
         for (int i = 0; i < MI; ++i)
             #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-        // scale bytes, 4 steps to a dword
-        const int ma = min(m0, g.M - 1) >> g.ash, na = min(n0, g.N - 1) >> g.bsh;
-        const uint8_t* base_as = g.as + (int64_t)ma * g.S;
-        const uint8_t* base_bs = g.bs + (int64_t)na * g.S;
-        uint32_t oa[MI], ob[4];
-        int ea[MI], eb[4];
-        #pragma unroll
-        for (int i = 0; i < MI; ++i)
-            oa[i] = ((min(m0 + i * 16 + l15, g.M - 1) >> g.ash) - ma) * g.S;
-        #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            ob[j] = ((min(n0 + (l15 >> 2) * 16 + j * 4 + (l15 & 3), g.N - 1) >>
-                      g.bsh) - na) * g.S;
+            for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+        int ea[MI], eb[NJ];
         for (int kb = 0; kb < g.nb; ++kb, buf ^= 1) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
             if ((kb & 3) == 0) {
+                sbuf ^= 1;
                 #pragma unroll
                 for (int i = 0; i < MI; ++i)
-                    ea[i] = *(const int*)(base_as + kb + oa[i]);
+                    ea[i] = lds_s[sbuf * (TM + TN) + wm + i * 16 + l15];
                 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    eb[j] = *(const int*)(base_bs + kb + ob[j]);
+                for (int j = 0; j < NJ; ++j)
+                    eb[j] = lds_s[sbuf * (TM + TN) + TM + wn + j * 16 + l15];
             } else {
                 #pragma unroll
                 for (int i = 0; i < MI; ++i) ea[i] >>= 8;
                 #pragma unroll
-                for (int j = 0; j < 4; ++j) eb[j] >>= 8;
+                for (int j = 0; j < NJ; ++j) eb[j] >>= 8;
             }
-            // the scales are waited for here, with the buffer: further down the
-            // compiler would wait for loads that are for the next step
-            #pragma unroll
-            for (int i = 0; i < MI; ++i) asm volatile("" : "+v"(ea[i]));
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(eb[j]));
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            // the other buffer: all waves are past reading it
-            if (kb + 1 < g.nb) {
-                stage(buf ^ 1, kb + 1);
-            } else if (tile + stride < end) {
-                enter(tile + stride);
-                stage(buf ^ 1, 0);
-            }
+            // The next step goes into the other buffer, which all waves are
+            // past reading; behind the last step the tile's first, for
+            // nothing.  Its loads are issued between the products of the
+            // first half of this step: a wave that issues them at once waits
+            // for the memory pipe to take them, and multiplies nothing.
+            const bool last = kb + 1 == g.nb;
+            if (last && tile + stride < end) enter(tile + stride);
+            const int next = last ? 0 : kb + 1;
+            constexpr int PER = 2 * (LA + LB) / MI;
             const uint8_t* A = lds + buf * BUF;
             const uint8_t* B = A + TM * 128;
             auto piece = [&](const uint8_t* base, int row, int p) {
                 return *(const i32x4*)(base + row * 128 +
                                        ((p ^ ((row >> 1) & 7)) * 16));
             };
+            auto row_a = [&](int i) {
+                return two(piece(A, wm + i * 16 + l15, l4),
+                           piece(A, wm + i * 16 + l15, 4 + l4));
+            };
             if (!EXACT) {
-                i32x8 fb[4];
+                // reads run two fragments ahead of the products
+                i32x8 fa[3], fb[NJ];
+                fa[0] = row_a(0);
                 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < NJ; ++j)
                     fb[j] = two(piece(B, wn + j * 16 + l15, l4),
                                 piece(B, wn + j * 16 + l15, 4 + l4));
-                i32x8 fa[2];
-                fa[0] = two(piece(A, wm + l15, l4), piece(A, wm + l15, 4 + l4));
+                fa[1] = row_a(1);
                 #pragma unroll
                 for (int i = 0; i < MI; ++i) {
-                    if (i + 1 < MI)
-                        fa[(i + 1) & 1] =
-                            two(piece(A, wm + (i + 1) * 16 + l15, l4),
-                                piece(A, wm + (i + 1) * 16 + l15, 4 + l4));
-                    __builtin_amdgcn_sched_barrier(0);  // read ahead
+                    if (i + 2 < MI) fa[(i + 2) % 3] = row_a(i + 2);
+                    stage(buf ^ 1, next, i * PER, (i + 1) * PER);
+                    __builtin_amdgcn_sched_barrier(0);
                     #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int j = 0; j < NJ; ++j)
                         acc[i][j] =
                             __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                                fb[j], fa[i & 1], acc[i][j], 0, 0, 0, eb[j], 0,
+                                fb[j], fa[i % 3], acc[i][j], 0, 0, 0, eb[j], 0,
                                 ea[i]);
                 }
             } else {
                 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    bf16x8 fb[4][2];
+                    bf16x8 fb[NJ][2];
+                    i32x4 fa[3];
+                    fa[0] = piece(A, wm + l15, h * 4 + l4);
                     #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < NJ; ++j) {
                         const i32x4 w = piece(B, wn + j * 16 + l15, h * 4 + l4);
                         fb[j][0] = expand8(w[0], w[1], eb[j] & 255);
                         fb[j][1] = expand8(w[2], w[3], eb[j] & 255);
                     }
+                    fa[1] = piece(A, wm + 16 + l15, h * 4 + l4);
                     #pragma unroll
                     for (int i = 0; i < MI; ++i) {
-                        const i32x4 w = piece(A, wm + i * 16 + l15, h * 4 + l4);
+                        if (i + 2 < MI)
+                            fa[(i + 2) % 3] =
+                                piece(A, wm + (i + 2) * 16 + l15, h * 4 + l4);
+                        if (h == 0) stage(buf ^ 1, next, i * PER / 2, (i + 1) * PER / 2);
+                        __builtin_amdgcn_sched_barrier(0);
+                        const i32x4 w = fa[i % 3];
                         const bf16x8 lo = expand8(w[0], w[1], ea[i] & 255);
                         const bf16x8 hi = expand8(w[2], w[3], ea[i] & 255);
                         #pragma unroll
-                        for (int j = 0; j < 4; ++j)
+                        for (int j = 0; j < NJ; ++j)
                             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                                 fb[j][0], lo, acc[i][j], 0, 0, 0);
                         #pragma unroll
-                        for (int j = 0; j < 4; ++j)
+                        for (int j = 0; j < NJ; ++j)
                             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                                 fb[j][1], hi, acc[i][j], 0, 0, 0);
                     }
                 }
             }
         }
-        // columns n ... n + 15 of rows m0 + 16 i + l15
-        const int n = n0 + l4 * 16;
-        float bias[16];
+        // columns n ... n + 15 of rows m0 + 16 i + l15, for each 64 columns
         #pragma unroll
-        for (int e = 0; e < 16; ++e) bias[e] = bias_at(g, min(n + e, g.N - 1));
-        const bool whole = n + 16 <= g.N && (g.N * sizeof(T) & 15) == 0;
-        #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const int m = m0 + i * 16 + l15;
-            unsigned bits = 0;
-            struct alignas(16) Pack { T t[16]; } p;
+        for (int c = 0; c < NJ / 4; ++c) {
+            const int n = n0 + c * 64 + l4 * 16;
+            if (n >= g.N) continue;
+            float bias[16];
             #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int e = 0; e < 16; ++e) bias[e] = bias_at(g, min(n + e, g.N - 1));
+            const bool whole = n + 16 <= g.N && (g.N * sizeof(T) & 15) == 0;
+            #pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                const int m = m0 + i * 16 + l15;
+                unsigned bits = 0;
+                struct alignas(16) Pack { T t[16]; } p;
                 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float z = acc[i][j][e] + bias[j * 4 + e];
-                    const bool on = passes(z);
-                    bits |= (unsigned)(on && n + j * 4 + e < g.N) << (j * 4 + e);
-                    if (g.relu && !on) z = 0.0f;
-                    p.t[j * 4 + e] = from_f<T>(z);
+                for (int j = 0; j < 4; ++j) {
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float z = acc[i][c * 4 + j][e] + bias[j * 4 + e];
+                        const bool on = passes(z);
+                        bits |= (unsigned)(on && n + j * 4 + e < g.N) << (j * 4 + e);
+                        if (g.relu && !on) z = 0.0f;
+                        p.t[j * 4 + e] = from_f<T>(z);
+                    }
                 }
-            }
-            if (m >= g.M || n >= g.N) continue;
-            if (g.mask)
-                *(uint16_t*)(g.mask + (int64_t)m * (((g.N + 127) >> 7) * 16) +
-                             (n >> 3)) = (uint16_t)bits;
-            T* out = (T*)g.c + (int64_t)m * g.N + n;
-            if (whole) {
-                *(Pack*)out = p;
-            } else {
-                #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (n + e < g.N) out[e] = p.t[e];
+                if (m >= g.M) continue;
+                if (g.mask)
+                    *(uint16_t*)(g.mask + (int64_t)m * (((g.N + 127) >> 7) * 16) +
+                                 (n >> 3)) = (uint16_t)bits;
+                T* out = (T*)g.c + (int64_t)m * g.N + n;
+                if (whole) {
+                    *(Pack*)out = p;
+                } else {
+                    #pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (n + e < g.N) out[e] = p.t[e];
+                }
             }
         }
     }
+    // no load may come in after the workgroup has given its LDS back
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #endif
 }
 
-template <int WM, int WN, int MI, typename T>
+template <int WM, int WN, int MI, int NJ, typename T>
 void launch_tiles(const Gemm& g, hipStream_t st) {
-    constexpr int TM = WM * MI * 16, TN = WN * 64;
-    constexpr int bytes = 2 * (TM + TN) * 128;
+    constexpr int TM = WM * MI * 16, TN = WN * NJ * 16;
+    constexpr int bytes = 2 * (TM + TN) * (128 + 4);
     const int64_t tiles =
         (int64_t)((g.M + TM - 1) / TM) * ((g.N + TN - 1) / TN);
     // as many workgroups as the 256 CUs hold, in whole rounds of the 8 XCDs
     const int64_t most = 256 * (163840 / bytes);
     const dim3 grid((uint32_t)min((tiles + 7) / 8 * 8, most));
     if (sizeof(T) == 4 || g.mask)
-        hipLaunchKernelGGL((gemm_tile_kernel<WM, WN, MI, true, T>), grid,
+        hipLaunchKernelGGL((gemm_tile_kernel<WM, WN, MI, NJ, true, T>), grid,
                            dim3(64 * WM * WN), bytes, st, g);
     else
-        hipLaunchKernelGGL((gemm_tile_kernel<WM, WN, MI, sizeof(T) == 4, T>),
+        hipLaunchKernelGGL((gemm_tile_kernel<WM, WN, MI, NJ, sizeof(T) == 4, T>),
                            grid, dim3(64 * WM * WN), bytes, st, g);
 }
 
@@ -1018,9 +1048,9 @@ int riqn_fp8_gemm(const uint8_t* a, const uint8_t* as, int a_block_rows,
             hipLaunchKernelGGL((gemm_direct_kernel<1, 1, T>), dim3(tiles),
                                dim3(512), 0, st, g);
         } else if ((int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 128) {
-            launch_tiles<2, 4, 8, T>(g, st);
+            launch_tiles<2, 4, 8, 4, T>(g, st);
         } else if ((int64_t)((M + 127) / 128) * ((N + 127) / 128) >= 128) {
-            launch_tiles<2, 2, 4, T>(g, st);
+            launch_tiles<2, 2, 4, 4, T>(g, st);
         } else {
             const int64_t tiles =
                 (int64_t)((M + 31) / 32) * ((N + 31) / 32);
