@@ -102,25 +102,36 @@ int row_groups(int64_t rows, int64_t rows_per_pass, int64_t most) {
                                   most);
 }
 
+Blocks new_blocks(const Tensor& like, int64_t R, int64_t C,
+                  int64_t block_rows) {
+    const int64_t nb = blocks_of(C);
+    return {torch::empty({R, nb * 128}, bytes_on(like)),
+            torch::empty({block_rows == 1 ? R : blocks_of(R), padded4(nb)},
+                         bytes_on(like)),
+            R, block_rows};
+}
+
+// workgroups of 4 waves that share out the rows of a strip of 4 blocks (or of
+// 1, where there are fewer than 4)
+int quant_groups(int64_t R, int64_t C, int64_t most) {
+    return row_groups(R, blocks_of(C) >= 4 ? 4 : 16, most);
+}
+
 // scale per 1 x 128 block; with `mask` values whose bit is clear count as
-// zero; `sum` (may be undefined) gets the sums of the columns
+// zero; `sum` (may be null) gets the sums of the columns
 Blocks quant_rows(const Tensor& x, const uint8_t* mask, Tensor* sum) {
     const int64_t R = x.size(0), C = x.size(1), nb = blocks_of(C);
-    Blocks o{torch::empty({R, nb * 128}, bytes_on(x)),
-             torch::empty({R, padded4(nb)}, bytes_on(x)), R, 1};
-    const bool wide = nb >= 4;
-    const int64_t strips = wide ? (nb + 3) / 4 : nb;
-    // every group leaves a row of partial sums to be added up: 1024
+    Blocks o = new_blocks(x, R, C, 1);
+    // with sums every group leaves a row of partial ones to be added up: 1024
     // workgroups in all fill the card and keep those few
-    const int groups =
-        row_groups(R, wide ? 4 : 16,
-                   sum ? std::max<int64_t>(1, 1024 / strips) : 65535);
+    const int64_t strips = nb >= 4 ? (nb + 3) / 4 : nb;
+    const int groups = quant_groups(
+        R, C, sum ? std::max<int64_t>(1, 1024 / strips) : 65535);
     Tensor part;
     if (sum) part = torch::empty({groups, C}, floats_on(x));
-    const int type = type_code(x.scalar_type(), "x");
     launched(riqn_fp8_quant_rows(
-                 x.data_ptr(), type, x.stride(0), mask,
-                 o.q.data_ptr<uint8_t>(), o.scale.data_ptr<uint8_t>(),
+                 x.data_ptr(), type_code(x.scalar_type(), "x"), x.stride(0),
+                 mask, o.q.data_ptr<uint8_t>(), o.scale.data_ptr<uint8_t>(),
                  sum ? part.data_ptr<float>() : nullptr, groups, (int)R,
                  (int)C, stream_of(x)),
              "quantize_fp8_blocks");
@@ -132,23 +143,21 @@ Blocks quant_rows(const Tensor& x, const uint8_t* mask, Tensor* sum) {
     return o;
 }
 
-// scale per 128 x 128 block, and the transposed matrix where `t` is given
-Blocks quant_tiles(const Tensor& x, Blocks* t) {
-    const int64_t R = x.size(0), C = x.size(1);
-    const int64_t nb = blocks_of(C), nbt = blocks_of(R);
-    TORCH_CHECK(nbt <= 65535, "a matrix with a scale per 128 x 128 block must "
-                "have at most 65535 blocks of rows");
-    Blocks o{torch::empty({R, nb * 128}, bytes_on(x)),
-             torch::empty({nbt, padded4(nb)}, bytes_on(x)), R, 128};
-    if (t)
-        *t = Blocks{torch::empty({C, nbt * 128}, bytes_on(x)),
-                    torch::empty({nb, padded4(nbt)}, bytes_on(x)), C, 128};
+void check_tiles(const Tensor& w) {
+    TORCH_CHECK(blocks_of(w.size(0)) <= 65535 &&
+                    blocks_of(w.size(0)) * blocks_of(w.size(1)) < (1 << 30),
+                "a matrix with a scale per 128 x 128 block must have at most "
+                "65535 blocks of rows and 2^30 blocks");
+}
+
+// scale per 128 x 128 block
+Blocks quant_tiles(const Tensor& x) {
+    check_tiles(x);
+    Blocks o = new_blocks(x, x.size(0), x.size(1), 128);
     launched(riqn_fp8_quant_tiles(
                  x.data_ptr(), type_code(x.scalar_type(), "x"), x.stride(0),
-                 o.q.data_ptr<uint8_t>(), o.scale.data_ptr<uint8_t>(),
-                 t ? t->q.data_ptr<uint8_t>() : nullptr,
-                 t ? t->scale.data_ptr<uint8_t>() : nullptr, (int)R, (int)C,
-                 stream_of(x)),
+                 o.q.data_ptr<uint8_t>(), o.scale.data_ptr<uint8_t>(), nullptr,
+                 nullptr, (int)x.size(0), (int)x.size(1), stream_of(x)),
              "quantize_fp8_blocks");
     return o;
 }
@@ -172,13 +181,9 @@ std::tuple<Tensor, Tensor> fp8_blocks_quant(Tensor x, int64_t block_rows) {
     TORCH_CHECK(block_rows == 1 || block_rows == 128, "block_rows must be 1 or 128");
     type_code(x.scalar_type(), "x");
     c10::cuda::CUDAGuard guard(x.device());
-    if (x.size(0) == 0) {
-        const int64_t nb = blocks_of(x.size(1));
-        return {torch::empty({0, nb * 128}, bytes_on(x)),
-                torch::empty({0, padded4(nb)}, bytes_on(x))};
-    }
-    Blocks o = block_rows == 1 ? quant_rows(x, nullptr, nullptr)
-                               : quant_tiles(x, nullptr);
+    Blocks o = x.size(0) == 0    ? new_blocks(x, 0, x.size(1), block_rows)
+               : block_rows == 1 ? quant_rows(x, nullptr, nullptr)
+                                 : quant_tiles(x);
     return {o.q, o.scale};
 }
 
@@ -265,26 +270,46 @@ Tensor linear_fwd(const Tensor& x, const Tensor& w, const OptTensor& bias,
         check_vector(*bias, w.size(0), x, "bias");
         type_code(bias->scalar_type(), "bias");
     }
-    type_code(x.scalar_type(), "x");
-    type_code(w.scalar_type(), "weight");
+    const int type = type_code(x.scalar_type(), "x");
+    const int w_type = type_code(w.scalar_type(), "weight");
+    check_tiles(w);
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t M = x.size(0), N = w.size(0), K = x.size(1);
     Tensor y = torch::empty({M, N}, x.options());
     if (M == 0 && !keep) return y;
-    Blocks wt;
-    Blocks wq = quant_tiles(w, need_dx ? &wt : nullptr);
+    Blocks xq = new_blocks(x, M, K, 1), wq = new_blocks(x, N, K, 128), wt;
+    uint8_t *wtq = nullptr, *wts = nullptr;
+    if (need_dx) {
+        wt = new_blocks(x, K, N, 128);
+        wtq = wt.q.data_ptr<uint8_t>();
+        wts = wt.scale.data_ptr<uint8_t>();
+    }
+    auto *xp = xq.q.data_ptr<uint8_t>(), *xsp = xq.scale.data_ptr<uint8_t>();
+    auto *wp = wq.q.data_ptr<uint8_t>(), *wsp = wq.scale.data_ptr<uint8_t>();
+    const int groups = quant_groups(M, K, 65535);
+    if (M > 0 && type == w_type) {
+        launched(riqn_fp8_quant_both(x.data_ptr(), x.stride(0), xp, xsp, groups,
+                                     (int)M, w.data_ptr(), w.stride(0), wp, wsp,
+                                     wtq, wts, (int)N, (int)K, type,
+                                     stream_of(x)),
+                 "linear_fp8_blocks");
+    } else {
+        if (M > 0)
+            launched(riqn_fp8_quant_rows(x.data_ptr(), type, x.stride(0),
+                                         nullptr, xp, xsp, nullptr, groups,
+                                         (int)M, (int)K, stream_of(x)),
+                     "linear_fp8_blocks");
+        launched(riqn_fp8_quant_tiles(w.data_ptr(), w_type, w.stride(0), wp,
+                                      wsp, wtq, wts, (int)N, (int)K,
+                                      stream_of(x)),
+                 "linear_fp8_blocks");
+    }
     Tensor bits;
     if (relu && keep)
         bits = torch::empty({M, blocks_of(N) * 16}, bytes_on(x));
-    Blocks xq;
-    if (M > 0) {
-        xq = quant_rows(x, nullptr, nullptr);
+    if (M > 0)
         gemm(xq, wq, K, bias, relu, y,
              bits.defined() ? bits.data_ptr<uint8_t>() : nullptr);
-    } else {
-        xq = {torch::empty({0, blocks_of(K) * 128}, bytes_on(x)),
-              torch::empty({0, padded4(blocks_of(K))}, bytes_on(x)), 0, 1};
-    }
     if (keep) *keep = {xq.q, xq.scale, wt.q, wt.scale, bits};
     return y;
 }
@@ -403,7 +428,16 @@ Tensor linear_fp8_serve(Tensor x0, Tensor wq, Tensor ws, int64_t block_rows,
     type_code(x.scalar_type(), "x");
     c10::cuda::CUDAGuard guard(x.device());
     Tensor y = torch::empty({x.size(0), w.rows}, x.options());
-    if (y.numel() > 0)
+    if (y.numel() > 0 && riqn_fp8_few(x.size(0), (int)x.size(1)))
+        launched(riqn_fp8_gemm_from(
+                     x.data_ptr(), type_code(x.scalar_type(), "x"), x.stride(0),
+                     w.q.data_ptr<uint8_t>(), w.scale.data_ptr<uint8_t>(),
+                     (int)block_rows, bias ? bias->data_ptr() : nullptr,
+                     bias ? type_code(bias->scalar_type(), "bias") : 0, relu,
+                     y.data_ptr(), (int)x.size(0), (int)w.rows, (int)x.size(1),
+                     stream_of(x)),
+                 "linear_fp8_blocks");
+    else if (y.numel() > 0)
         gemm(quant_rows(x, nullptr, nullptr), w, x.size(1), bias, relu, y,
              nullptr);
     return y.view(with_last(x0, w.rows));

@@ -22,6 +22,7 @@
 #include "riqn_kernels.h"
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
+#include <type_traits>
 
 namespace {
 
@@ -122,20 +123,19 @@ DEV void load8(const T* p, int col, int C, float* v) {
 // its partial sums in fp32 to part[blockIdx.y][C]; no atomics, so the result
 // does not depend on the order in which workgroups run.
 // ---------------------------------------------------------------------------
-template <typename T, bool VEC, int BPW, bool MASK, bool SUM>
-__global__ __launch_bounds__(256) void quant_rows_kernel(
-    const T* __restrict__ x, int64_t ldx, const uint8_t* __restrict__ mask,
-    uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
-    float* __restrict__ part, int R, int C, int nb, int S) {
+template <typename T, bool VEC, int BPW, bool MASK, bool SUM, int WAVES>
+DEV void quant_rows(const T* __restrict__ x, int64_t ldx,
+                    const uint8_t* __restrict__ mask, uint8_t* __restrict__ q,
+                    uint8_t* __restrict__ scale, int R, int C, int nb, int S,
+                    int strip, int group, int groups, float (&sum)[8]) {
     constexpr int RPW = 4 / BPW;  // rows of a wave
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int grp = lane >> 4, l15 = lane & 15;
-    const int blk = blockIdx.x * BPW + (BPW == 4 ? grp : 0);
+    const int blk = strip * BPW + (BPW == 4 ? grp : 0);
     const int col = blk * 128 + l15 * 8;
-    const int step = 4 * RPW * gridDim.y;
-    float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const int step = WAVES * RPW * groups;
     if (blk < nb) {
-        for (int r = (blockIdx.y * 4 + wave) * RPW + (BPW == 4 ? 0 : grp);
+        for (int r = (group * WAVES + wave) * RPW + (BPW == 4 ? 0 : grp);
              r < R; r += step) {
             float v[8];
             load8<T, VEC>(x + r * ldx, col, C, v);
@@ -159,6 +159,19 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(
                 for (int i = nb; i < S; ++i) scale[(int64_t)r * S + i] = 0;
         }
     }
+}
+
+template <typename T, bool VEC, int BPW, bool MASK, bool SUM>
+__global__ __launch_bounds__(256) void quant_rows_kernel(
+    const T* __restrict__ x, int64_t ldx, const uint8_t* __restrict__ mask,
+    uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
+    float* __restrict__ part, int R, int C, int nb, int S) {
+    constexpr int RPW = 4 / BPW;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    quant_rows<T, VEC, BPW, MASK, SUM, 4>(x, ldx, mask, q, scale, R, C, nb, S,
+                                          blockIdx.x, blockIdx.y, gridDim.y,
+                                          sum);
     if (SUM) {
         __shared__ float red[4][64][9];  // 9: lanes on different banks
         #pragma unroll
@@ -202,25 +215,32 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(
 // ---------------------------------------------------------------------------
 // Quantisation with a scale per 128 x 128 block, for weights; qt/scale_t (may
 // be null) get the transposed matrix, whose blocks have the same scales.  One
-// workgroup per block: 64 values a thread stay in registers between the
+// workgroup per block: 32 values a thread stay in registers between the
 // maximum and the conversion; the transposed bytes go through LDS.
 // ---------------------------------------------------------------------------
+struct Tiles {
+    const void* x;           // [R, C] of T, rows ldx apart
+    int64_t ldx;
+    uint8_t *q, *scale, *qt, *scale_t;
+    int R, C, nb, S, nbt, St;
+};
+
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void quant_tiles_kernel(
-    const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
-    uint8_t* __restrict__ scale, uint8_t* __restrict__ qt,
-    uint8_t* __restrict__ scale_t, int R, int C, int nb, int S, int nbt,
-    int St) {
-    __shared__ float wmax[4];
+DEV void quant_tile(const Tiles& a, int bc, int br) {
+    __shared__ float wmax[8];
     __shared__ uint8_t tile[128][132];  // 132: columns fall on all banks
     const int t = threadIdx.x, l15 = t & 15, rr = t >> 4;
-    const int bc = blockIdx.x, br = blockIdx.y;
+    const T* const x = (const T*)a.x;
+    const int64_t ldx = a.ldx;
+    uint8_t *const q = a.q, *const scale = a.scale, *const qt = a.qt,
+            *const scale_t = a.scale_t;
+    const int R = a.R, C = a.C, nb = a.nb, S = a.S, nbt = a.nbt, St = a.St;
     const int col = bc * 128 + l15 * 8;
-    float v[8][8];
+    float v[4][8];
     float am = 0.0f;
     #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = br * 128 + i * 16 + rr;
+    for (int i = 0; i < 4; ++i) {
+        const int r = br * 128 + i * 32 + rr;
         if (r < R) {
             load8<T, VEC>(x + r * ldx, col, C, v[i]);
         } else {
@@ -234,17 +254,18 @@ __global__ __launch_bounds__(256) void quant_tiles_kernel(
     for (int off = 32; off > 0; off >>= 1) am = fmaxf(am, __shfl_xor(am, off, 64));
     if ((t & 63) == 0) wmax[t >> 6] = am;
     __syncthreads();
-    am = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) am = fmaxf(am, wmax[i]);
     const int e = block_exp(am);
     const float inv = pow2i(-e);
     #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = br * 128 + i * 16 + rr;
+    for (int i = 0; i < 4; ++i) {
+        const int r = br * 128 + i * 32 + rr;
         const i32x2 w = pack8(v[i], inv);
         if (r < R) *(i32x2*)(q + (int64_t)r * (nb * 128) + col) = w;
         if (qt) {
-            *(int*)&tile[i * 16 + rr][l15 * 8] = w[0];
-            *(int*)&tile[i * 16 + rr][l15 * 8 + 4] = w[1];
+            *(int*)&tile[i * 32 + rr][l15 * 8] = w[0];
+            *(int*)&tile[i * 32 + rr][l15 * 8 + 4] = w[1];
         }
     }
     if (t == 0) {
@@ -259,11 +280,10 @@ __global__ __launch_bounds__(256) void quant_tiles_kernel(
     }
     if (!qt) return;
     __syncthreads();
-    // 8 rows x 4 columns a turn, transposed by byte permutes; 16 lanes write
+    // 8 rows x 4 columns a thread, transposed by byte permutes; 16 lanes write
     // the 128 bytes of one row of the transposed block
-    #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int n8 = t & 15, c4 = i * 16 + (t >> 4);
+    {
+        const int n8 = t & 15, c4 = t >> 4;
         uint32_t d[8], o[4][2];
         #pragma unroll
         for (int r = 0; r < 8; ++r)
@@ -271,12 +291,12 @@ __global__ __launch_bounds__(256) void quant_tiles_kernel(
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t* e = d + 4 * h;
-            const uint32_t a = __builtin_amdgcn_perm(e[1], e[0], 0x05010400);
+            const uint32_t aa = __builtin_amdgcn_perm(e[1], e[0], 0x05010400);
             const uint32_t b = __builtin_amdgcn_perm(e[1], e[0], 0x07030602);
             const uint32_t u = __builtin_amdgcn_perm(e[3], e[2], 0x05010400);
             const uint32_t v = __builtin_amdgcn_perm(e[3], e[2], 0x07030602);
-            o[0][h] = __builtin_amdgcn_perm(u, a, 0x05040100);
-            o[1][h] = __builtin_amdgcn_perm(u, a, 0x07060302);
+            o[0][h] = __builtin_amdgcn_perm(u, aa, 0x05040100);
+            o[1][h] = __builtin_amdgcn_perm(u, aa, 0x07060302);
             o[2][h] = __builtin_amdgcn_perm(v, b, 0x05040100);
             o[3][h] = __builtin_amdgcn_perm(v, b, 0x07060302);
         }
@@ -287,6 +307,29 @@ __global__ __launch_bounds__(256) void quant_tiles_kernel(
                 *(i32x2*)(qt + (int64_t)c * (nbt * 128) + br * 128 + n8 * 8) =
                     i32x2{(int)o[r][0], (int)o[r][1]};
         }
+    }
+}
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(512) void quant_tiles_kernel(Tiles a) {
+    quant_tile<T, VEC>(a, blockIdx.x, blockIdx.y);
+}
+
+// A weight's tiles and an activation's rows in one launch, the forward pass of
+// a training step: the first `tiles` workgroups take the weight.
+template <typename T, int BPW>
+__global__ __launch_bounds__(512) void quant_both_kernel(
+    Tiles a, const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
+    uint8_t* __restrict__ scale, int R, int nb, int S, int tiles, int strips,
+    int groups) {
+    if ((int)blockIdx.x < tiles) {
+        quant_tile<T, true>(a, blockIdx.x % nb, blockIdx.x / nb);
+    } else {
+        const int id = blockIdx.x - tiles;
+        float none[8];
+        quant_rows<T, true, BPW, false, false, 8>(
+            x, ldx, nullptr, q, scale, R, a.C, nb, S, id % strips, id / strips,
+            groups, none);
     }
 }
 
@@ -336,6 +379,9 @@ struct Gemm {
     void* c;                         // [M, N]
     uint8_t* mask;                   // [M, 16 ceil(N / 128)] bits, or null
     int M, N, nb, S, ash, bsh, bias_t, relu;
+    const void* x;                   // [M, K], rows ldx apart, in place of a
+    int64_t ldx;
+    int K;
 };
 
 DEV float bias_at(const Gemm& g, int n) {
@@ -355,6 +401,49 @@ DEV bf16x8 expand8(int w0, int w1, int sbyte) {
     u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, false);
     u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, true);
     return u.v;
+}
+
+// adds the partial tiles of 8 waves in a fixed order and stores the result
+template <int TM, int TN, typename T>
+DEV void finish_direct(const Gemm& g, float (&red)[8][TM][TN + 4], int m0,
+                       int n0) {
+    const int t = threadIdx.x;
+    __syncthreads();
+    constexpr int QUADS = TM * TN / 4;
+    if (t >= QUADS) return;
+    const int mm = t / (TN / 4), nn = (t % (TN / 4)) * 4;
+    f32x4 z = *(const f32x4*)&red[0][mm][nn];
+    #pragma unroll
+    for (int w = 1; w < 8; ++w) z += *(const f32x4*)&red[w][mm][nn];
+    const int m = m0 + mm, n = n0 + nn;
+    unsigned bits = 0;
+    struct alignas(4 * sizeof(T)) Pack { T t[4]; } p;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float y = z[j] + (n + j < g.N ? bias_at(g, n + j) : 0.0f);
+        const bool on = passes(y);
+        bits |= (unsigned)(on && n + j < g.N) << j;
+        if (g.relu && !on) y = 0.0f;
+        p.t[j] = from_f<T>(y);
+    }
+    if (g.mask) {
+        // four neighbours make 16 columns; quads of a row are 4-aligned
+        bits <<= 4 * (t & 3);
+        bits |= __shfl_xor(bits, 1, 64);
+        bits |= __shfl_xor(bits, 2, 64);
+        if ((t & 3) == 0 && m < g.M)
+            *(uint16_t*)(g.mask + (int64_t)m * (((g.N + 127) >> 7) * 16) +
+                         (n >> 3)) = (uint16_t)bits;
+    }
+    if (m >= g.M) return;
+    T* out = (T*)g.c + (int64_t)m * g.N + n;
+    if ((g.N & 3) == 0) {
+        if (n < g.N) *(Pack*)out = p;
+    } else {
+        #pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (n + j < g.N) out[j] = p.t[j];
+    }
 }
 
 // Few rows or small results: a workgroup of 8 waves computes a tile of
@@ -432,42 +521,67 @@ __global__ __launch_bounds__(512) void gemm_direct_kernel(Gemm g) {
         #pragma unroll
         for (int j = 0; j < NI; ++j)
             *(f32x4*)&red[wave][i * 16 + l15][j * 16 + l4 * 4] = acc[i][j];
-    __syncthreads();
-    constexpr int QUADS = TM * TN / 4;
-    if (t >= QUADS) return;
-    const int mm = t / (TN / 4), nn = (t % (TN / 4)) * 4;
-    f32x4 z = *(const f32x4*)&red[0][mm][nn];
-    #pragma unroll
-    for (int w = 1; w < 8; ++w) z += *(const f32x4*)&red[w][mm][nn];
-    const int m = m0 + mm, n = n0 + nn;
-    unsigned bits = 0;
-    struct alignas(4 * sizeof(T)) Pack { T t[4]; } p;
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        float y = z[j] + (n + j < g.N ? bias_at(g, n + j) : 0.0f);
-        const bool on = passes(y);
-        bits |= (unsigned)(on && n + j < g.N) << j;
-        if (g.relu && !on) y = 0.0f;
-        p.t[j] = from_f<T>(y);
-    }
-    if (g.mask) {
-        // four neighbours make 16 columns; quads of a row are 4-aligned
-        bits <<= 4 * (t & 3);
-        bits |= __shfl_xor(bits, 1, 64);
-        bits |= __shfl_xor(bits, 2, 64);
-        if ((t & 3) == 0 && m < g.M)
-            *(uint16_t*)(g.mask + (int64_t)m * (((g.N + 127) >> 7) * 16) +
-                         (n >> 3)) = (uint16_t)bits;
-    }
-    if (m >= g.M) return;
-    T* out = (T*)g.c + (int64_t)m * g.N + n;
-    if ((g.N & 3) == 0) {
-        if (n < g.N) *(Pack*)out = p;
-    } else {
+    finish_direct<TM, TN, T>(g, red, m0, n0);
+}
+
+// A product of up to 16 rows that are not in 8 bits yet, for serving: one
+// launch instead of two, which is what such a call takes its time with.  The
+// workgroup first quantises the rows into LDS, exactly as quant_rows_kernel
+// does, while its first piece of B is on the way; then as above.
+// [1, 1024, 3136]: 5.7 us a call, 10.4 by two launches.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(512) void gemm_few_kernel(Gemm g) {
+    __shared__ float red[8][16][20];
+    extern __shared__ __align__(16) uint8_t lds[];  // rows, then their scales
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int l15 = lane & 15, l4 = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const int pitch = g.nb * 128 + 16;  // 16: rows begin on different banks
+    uint8_t* const scales = lds + g.M * pitch;
+    const int64_t rb = min(n0 + l15, g.N - 1);
+    const uint8_t* pb = g.b + rb * ((int64_t)g.nb * 128) + l4 * 16;
+    const uint8_t* sb = g.bs + (rb >> g.bsh) * g.S;
+    i32x4 fb[2];
+    int eb = 0;
+    auto load = [&](int kb) {
+        fb[0] = *(const i32x4*)(pb + kb * 128);
+        fb[1] = *(const i32x4*)(pb + kb * 128 + 64);
+        eb = sb[kb];
+    };
+    load(min(wave, g.nb - 1));
+    for (int i = t >> 4; i < g.M * g.nb; i += 32) {
+        const int r = i / g.nb, blk = i - r * g.nb;
+        float v[8];
+        load8<T, VEC>((const T*)g.x + r * g.ldx, blk * 128 + l15 * 8, g.K, v);
+        float am = 0.0f;
         #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (n + j < g.N) out[j] = p.t[j];
+        for (int j = 0; j < 8; ++j) am = fmaxf(am, finite_abs(v[j]));
+        const int e = block_exp(max16(am));
+        *(i32x2*)(lds + r * pitch + blk * 128 + l15 * 8) = pack8(v, pow2i(-e));
+        if (l15 == 0) scales[i] = (uint8_t)(e + 127);
     }
+    __syncthreads();
+    const int ra = min(l15, g.M - 1);
+    f32x4 acc = {0, 0, 0, 0};
+    for (int kb = wave; kb < g.nb; kb += 8) {
+        const i32x4 b0 = fb[0], b1 = fb[1];
+        const int e1 = eb;
+        load(min(kb + 8, g.nb - 1));  // the next piece
+        const uint8_t* p = lds + ra * pitch + kb * 128 + l4 * 16;
+        const i32x4 a0 = *(const i32x4*)p, a1 = *(const i32x4*)(p + 64);
+        const int e0 = scales[ra * g.nb + kb];
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const i32x4 a = h ? a1 : a0, b = h ? b1 : b0;
+            #pragma unroll
+            for (int u = 0; u < 4; u += 2)
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    expand8(b[u], b[u + 1], e1), expand8(a[u], a[u + 1], e0),
+                    acc, 0, 0, 0);
+        }
+    }
+    *(f32x4*)&red[wave][l15][l4 * 4] = acc;
+    finish_direct<16, 16, T>(g, red, 0, n0);
 }
 
 // ---------------------------------------------------------------------------
@@ -479,9 +593,10 @@ __global__ __launch_bounds__(512) void gemm_direct_kernel(Gemm g) {
 //
 // LDS rows are 128 bytes; the 16-byte piece p of row r lies at p ^ (r / 2 % 8),
 // so the 16 rows that a fragment reads fall on all 64 banks.  B's rows lie in
-// the order in which lane group l4 of fragment i gets columns 16 l4 + 4 i ...:
-// a lane then ends up with 16 neighbours of one row of C, 32 bytes to store
-// and 16 bits for the relu.
+// the order in which lane group l4 of a pair of fragments gets columns 8 l4
+// ... 8 l4 + 7 of 32: a lane then ends up with 8 neighbours of one row of C,
+// the 4 groups with 32, and a store of 16 bits a value fills 64 bytes of each
+// of 16 rows.
 //
 // EXACT: operands expanded to bf16, every product summed in full, for results
 // in fp32 and where a relu's bits decide gradients.  Otherwise the scaled
@@ -506,7 +621,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
     // [2][BUF] tiles, [2][TM + TN] dwords of scales
     extern __shared__ __align__(16) uint8_t lds[];
     uint32_t* const lds_s = (uint32_t*)(lds + 2 * BUF);
-    static_assert(TM + TN == 64 * WAVES, "a scale a lane");
+    static_assert(TM + TN <= 64 * WAVES && TM % 64 == 0, "a scale a lane");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l15 = lane & 15, l4 = lane >> 4;
@@ -531,7 +646,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
     uint32_t off[LA + LB], off_s;
     // B's row at place r of a tile, see above
     auto place = [](int r) {
-        return (r & ~63) + ((r & 15) >> 2) * 16 + ((r >> 4) & 3) * 4 + (r & 3);
+        return (r & ~31) + ((r & 15) >> 2) * 8 + ((r >> 4) & 1) * 4 + (r & 3);
     };
     auto enter = [&](int tile) {
         const int m0 = (tile / nt) * TM, n0 = (tile % nt) * TN;
@@ -557,14 +672,14 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
             const int r0 = n0 >> g.bsh;
             buf_s = buffer_of(g.bs + (int64_t)r0 * g.S,
                               (((g.N - 1) >> g.bsh) + 1 - r0) * (int64_t)g.S);
-            off_s = ((min(n0 + place(r - TM), g.N - 1) >> g.bsh) - r0) * g.S;
+            off_s = (((n0 + min(place(r - TM), g.N - 1 - n0)) >> g.bsh) - r0) * g.S;
         }
     };
     int sbuf = 1;  // which scales are in use
     // loads [from, to) of a wave's share of a step
     auto stage = [&](int buf, int kb, int from, int to) {
         // the scales of 4 steps are a dword a row
-        if (from == 0 && (kb & 3) == 0)
+        if (from == 0 && (kb & 3) == 0 && wave * 64 < TM + TN)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 buf_s,
                 (__attribute__((address_space(3))) void*)(
@@ -583,6 +698,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
     };
     enter(tile);
     stage(0, 0, 0, LA + LB);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     int buf = 0;
     for (; tile < end; tile += stride) {
         const int m0 = (tile / nt) * TM + wm, n0 = (tile % nt) * TN + wn;
@@ -593,7 +709,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
             for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
         int ea[MI], eb[NJ];
         for (int kb = 0; kb < g.nb; ++kb, buf ^= 1) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            // a tile's first step was waited for before the last one's stores
+            if (kb > 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             if ((kb & 3) == 0) {
@@ -685,44 +802,59 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
                 }
             }
         }
-        // columns n ... n + 15 of rows m0 + 16 i + l15, for each 64 columns
-        #pragma unroll
-        for (int c = 0; c < NJ / 4; ++c) {
-            const int n = n0 + c * 64 + l4 * 16;
-            if (n >= g.N) continue;
-            float bias[16];
-            #pragma unroll
-            for (int e = 0; e < 16; ++e) bias[e] = bias_at(g, min(n + e, g.N - 1));
-            const bool whole = n + 16 <= g.N && (g.N * sizeof(T) & 15) == 0;
+        // The next tile's first step is waited for here: behind the stores it
+        // would be waited for with them, as the counter knows one order only.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // columns n ... n + 7 of rows m0 + 16 i + l15, for each 32 columns; a
+        // row's stores follow each other, so that whole lines are written
+        const bool even = (g.N & 7) == 0;  // all 8 there, and aligned
+        auto finish = [&](auto plain, const float (&bias)[NJ / 2][8]) {
             #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 const int m = m0 + i * 16 + l15;
-                unsigned bits = 0;
-                struct alignas(16) Pack { T t[16]; } p;
                 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int c = 0; c < NJ / 2; ++c) {
+                    const int n = n0 + c * 32 + l4 * 8;
+                    unsigned bits = 0;
+                    struct alignas(16) Pack { T t[8]; } p;
                     #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float z = acc[i][c * 4 + j][e] + bias[j * 4 + e];
-                        const bool on = passes(z);
-                        bits |= (unsigned)(on && n + j * 4 + e < g.N) << (j * 4 + e);
-                        if (g.relu && !on) z = 0.0f;
-                        p.t[j * 4 + e] = from_f<T>(z);
+                    for (int e = 0; e < 8; ++e) {
+                        float z = acc[i][c * 2 + (e >> 2)][e & 3];
+                        if (!decltype(plain)::value) {
+                            z += bias[c][e];
+                            const bool on = passes(z);
+                            bits |= (unsigned)(on && n + e < g.N) << e;
+                            if (g.relu && !on) z = 0.0f;
+                        }
+                        p.t[e] = from_f<T>(z);
+                    }
+                    if (m >= g.M || n >= g.N) continue;
+                    if (!decltype(plain)::value && g.mask)
+                        g.mask[(int64_t)m * (((g.N + 127) >> 7) * 16) + (n >> 3)] =
+                            (uint8_t)bits;
+                    T* out = (T*)g.c + (int64_t)m * g.N + n;
+                    if (even) {
+                        *(Pack*)out = p;
+                    } else {
+                        #pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (n + e < g.N) out[e] = p.t[e];
                     }
                 }
-                if (m >= g.M) continue;
-                if (g.mask)
-                    *(uint16_t*)(g.mask + (int64_t)m * (((g.N + 127) >> 7) * 16) +
-                                 (n >> 3)) = (uint16_t)bits;
-                T* out = (T*)g.c + (int64_t)m * g.N + n;
-                if (whole) {
-                    *(Pack*)out = p;
-                } else {
-                    #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (n + e < g.N) out[e] = p.t[e];
-                }
             }
+        };
+        // without any of them the results go out as they are: the rest is 10
+        // instructions a value, as long as 4 steps of products
+        float bias[NJ / 2][8];
+        if (g.bias || g.relu || g.mask) {
+            #pragma unroll
+            for (int c = 0; c < NJ / 2; ++c)
+                #pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    bias[c][e] = bias_at(g, min(n0 + c * 32 + l4 * 8 + e, g.N - 1));
+            finish(std::false_type{}, bias);
+        } else {
+            finish(std::true_type{}, bias);
         }
     }
     // no load may come in after the workgroup has given its LDS back
@@ -993,22 +1125,58 @@ int riqn_column_sum(const float* part, void* out, int type, int G, int C,
     return (int)hipGetLastError();
 }
 
+static Tiles tiles_of(const void* x, int64_t ldx, uint8_t* q, uint8_t* scale,
+                      uint8_t* qt, uint8_t* scale_t, int R, int C) {
+    const int nb = (C + 127) >> 7, nbt = (R + 127) >> 7;
+    return {x, ldx, q, scale, qt, scale_t, R, C, nb, (nb + 3) & ~3, nbt,
+            (nbt + 3) & ~3};
+}
+
 int riqn_fp8_quant_tiles(const void* x, int type, int64_t ldx, uint8_t* q,
                          uint8_t* scale, uint8_t* qt, uint8_t* scale_t, int R,
                          int C, void* stream) {
-    const int nb = (C + 127) >> 7, nbt = (R + 127) >> 7;
-    const bool vec = vec8(x, ldx, C, type);
+    const Tiles a = tiles_of(x, ldx, q, scale, qt, scale_t, R, C);
+    hipStream_t st = (hipStream_t)stream;
     RIQN_TYPE(type, T, {
-        if (vec)
-            hipLaunchKernelGGL((quant_tiles_kernel<T, true>), dim3(nb, nbt),
-                               dim3(256), 0, (hipStream_t)stream, (const T*)x,
-                               ldx, q, scale, qt, scale_t, R, C, nb,
-                               (nb + 3) & ~3, nbt, (nbt + 3) & ~3);
+        if (vec8(x, ldx, C, type))
+            hipLaunchKernelGGL((quant_tiles_kernel<T, true>), dim3(a.nb, a.nbt),
+                               dim3(512), 0, st, a);
         else
-            hipLaunchKernelGGL((quant_tiles_kernel<T, false>), dim3(nb, nbt),
-                               dim3(256), 0, (hipStream_t)stream, (const T*)x,
-                               ldx, q, scale, qt, scale_t, R, C, nb,
-                               (nb + 3) & ~3, nbt, (nbt + 3) & ~3);
+            hipLaunchKernelGGL((quant_tiles_kernel<T, false>),
+                               dim3(a.nb, a.nbt), dim3(512), 0, st, a);
+    })
+    return (int)hipGetLastError();
+}
+
+// x [M, C] by rows and w [N, C] by tiles, both of one type; where they are not
+// laid out for it, by two launches
+int riqn_fp8_quant_both(const void* x, int64_t ldx, uint8_t* xq, uint8_t* xs,
+                        int groups, int M, const void* w, int64_t ldw,
+                        uint8_t* wq, uint8_t* ws, uint8_t* wtq, uint8_t* wts,
+                        int N, int C, int type, void* stream) {
+    if (!vec8(x, ldx, C, type) || !vec8(w, ldw, C, type)) {
+        const int err = riqn_fp8_quant_rows(x, type, ldx, nullptr, xq, xs,
+                                            nullptr, groups, M, C, stream);
+        return err ? err
+                   : riqn_fp8_quant_tiles(w, type, ldw, wq, ws, wtq, wts, N, C,
+                                          stream);
+    }
+    const Tiles a = tiles_of(w, ldw, wq, ws, wtq, wts, N, C);
+    const bool wide = a.nb >= 4;
+    const int tiles = a.nb * a.nbt, strips = wide ? (a.nb + 3) / 4 : a.nb;
+    const int half = (groups + 1) / 2;  // 8 waves here, 4 there
+    hipStream_t st = (hipStream_t)stream;
+    RIQN_TYPE(type, T, {
+        if (wide)
+            hipLaunchKernelGGL((quant_both_kernel<T, 4>),
+                               dim3(tiles + strips * half), dim3(512), 0, st, a,
+                               (const T*)x, ldx, xq, xs, M, a.nb, a.S, tiles,
+                               strips, half);
+        else
+            hipLaunchKernelGGL((quant_both_kernel<T, 1>),
+                               dim3(tiles + strips * half), dim3(512), 0, st, a,
+                               (const T*)x, ldx, xq, xs, M, a.nb, a.S, tiles,
+                               strips, half);
     })
     return (int)hipGetLastError();
 }
@@ -1040,23 +1208,64 @@ int riqn_fp8_gemm(const uint8_t* a, const uint8_t* as, int a_block_rows,
     const int nb = (K + 127) >> 7;
     Gemm g{a, as, b, bs, bias, c, mask, M, N, nb, (nb + 3) & ~3,
            a_block_rows == 128 ? 7 : 0, b_block_rows == 128 ? 7 : 0, bias_type,
-           relu};
+           relu, nullptr, 0, K};
     hipStream_t st = (hipStream_t)stream;
+    auto tiles = [&](int t) {
+        return (int64_t)((M + t - 1) / t) * ((N + t - 1) / t);
+    };
+    // The largest tile of which there are enough for the 256 CUs: it moves the
+    // fewest bytes.  Measured in us, tiles of 32 (direct) / 64 / 128 / 256, in
+    // bf16, [M, 1024, 3136]: M = 256: 9 / 12 / 19 / 43, 512: 16 / 12 / 19 / 43,
+    // 4096: 102 / 25 / 25 / 44, 8192: - / 47 / 35 / 48, 16384: - / 91 / 61 /
+    // 54; [M, 3136, 1024]: M = 64: 5 / 6 / 9 / 15, 256: 11 / 6 / 10 / 25,
+    // 1024: 30 / 13 / 12 / 25, 4096: 97 / 33 / 30 / 28.
     RIQN_TYPE(c_type, T, {
         if (M <= 16) {
-            const uint32_t tiles = (N + 15) / 16;
-            hipLaunchKernelGGL((gemm_direct_kernel<1, 1, T>), dim3(tiles),
-                               dim3(512), 0, st, g);
-        } else if ((int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 128) {
+            hipLaunchKernelGGL((gemm_direct_kernel<1, 1, T>),
+                               dim3((N + 15) / 16), dim3(512), 0, st, g);
+        } else if (tiles(256) >= 192) {
             launch_tiles<2, 4, 8, 4, T>(g, st);
-        } else if ((int64_t)((M + 127) / 128) * ((N + 127) / 128) >= 128) {
+        } else if (tiles(128) >= 192) {
             launch_tiles<2, 2, 4, 4, T>(g, st);
+        } else if (tiles(32) > 256) {
+            launch_tiles<2, 2, 2, 2, T>(g, st);
         } else {
-            const int64_t tiles =
-                (int64_t)((M + 31) / 32) * ((N + 31) / 32);
             hipLaunchKernelGGL((gemm_direct_kernel<2, 2, T>),
-                               dim3((uint32_t)tiles), dim3(512), 0, st, g);
+                               dim3((uint32_t)tiles(32)), dim3(512), 0, st, g);
         }
+    })
+    return (int)hipGetLastError();
+}
+
+// LDS that riqn_fp8_gemm_from takes for M rows of K columns
+static int few_bytes(int64_t M, int K) {
+    const int nb = (K + 127) >> 7;
+    return (int)min(M * (nb * 128 + 16 + nb), (int64_t)1 << 30);
+}
+
+// whether a product of M rows that are not in 8 bits goes by one kernel
+int riqn_fp8_few(int64_t M, int K) {
+    return M <= 16 && few_bytes(M, K) <= 65536;
+}
+
+// the product of a few rows that are not in 8 bits yet; c has x's type
+int riqn_fp8_gemm_from(const void* x, int type, int64_t ldx, const uint8_t* b,
+                       const uint8_t* bs, int b_block_rows, const void* bias,
+                       int bias_type, int relu, void* c, int M, int N, int K,
+                       void* stream) {
+    const int nb = (K + 127) >> 7;
+    Gemm g{nullptr, nullptr, b, bs, bias, c, nullptr, M, N, nb, (nb + 3) & ~3,
+           0, b_block_rows == 128 ? 7 : 0, bias_type, relu, x, ldx, K};
+    const dim3 grid((N + 15) / 16);
+    const int bytes = few_bytes(M, K);
+    hipStream_t st = (hipStream_t)stream;
+    RIQN_TYPE(type, T, {
+        if (vec8(x, ldx, K, type))
+            hipLaunchKernelGGL((gemm_few_kernel<T, true>), grid, dim3(512),
+                               bytes, st, g);
+        else
+            hipLaunchKernelGGL((gemm_few_kernel<T, false>), grid, dim3(512),
+                               bytes, st, g);
     })
     return (int)hipGetLastError();
 }

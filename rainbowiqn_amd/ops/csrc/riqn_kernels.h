@@ -164,6 +164,10 @@ int riqn_column_sum(const float* part, void* out, int type, int G, int C,
 int riqn_fp8_quant_tiles(const void* x, int type, int64_t ldx, uint8_t* q,
                          uint8_t* scale, uint8_t* qt, uint8_t* scale_t, int R,
                          int C, void* stream);
+int riqn_fp8_quant_both(const void* x, int64_t ldx, uint8_t* xq, uint8_t* xs,
+                        int groups, int M, const void* w, int64_t ldw,
+                        uint8_t* wq, uint8_t* ws, uint8_t* wtq, uint8_t* wts,
+                        int N, int C, int type, void* stream);
 int riqn_fp8_dequant(const uint8_t* q, const uint8_t* scale, void* out,
                      int type, int R, int C, int shift, void* stream);
 int riqn_fp8_gemm(const uint8_t* a, const uint8_t* as, int a_block_rows,
@@ -171,6 +175,11 @@ int riqn_fp8_gemm(const uint8_t* a, const uint8_t* as, int a_block_rows,
                   const void* bias, int bias_type, int relu, void* c,
                   int c_type, uint8_t* mask, int M, int N, int K,
                   void* stream);
+int riqn_fp8_few(int64_t M, int K);
+int riqn_fp8_gemm_from(const void* x, int type, int64_t ldx, const uint8_t* b,
+                       const uint8_t* bs, int b_block_rows, const void* bias,
+                       int bias_type, int relu, void* c, int M, int N, int K,
+                       void* stream);
 int riqn_fp8_wgrad(const uint8_t* g, const uint8_t* gs, const uint8_t* x,
                    const uint8_t* xs, void* dw, int type, float* part,
                    int shares, int M, int N, int K, void* stream);
