@@ -86,6 +86,9 @@ class Config:
     fused_forward: bool = True  # hand-written fused model-forward kernels
     fused_backward: bool = True  # hand-written learn-step backward kernels
     fp8_heads: bool = False  # MX-fp8 NoisyLinear heads GEMM (config 5 path)
+    layer_norm: bool = False  # normalise the heads' input (tau-weighted features)
+    fp8_train: bool = False  # heads' hidden layer on 8-bit blocks, forward and
+    # backward; its input is kept in 8 bits for the backward pass
     overlap_colocated: bool = True  # actor/learner stream concurrency on 1 GPU
     cu_split: int = 96  # colocated overlap: CUs [0,N) -> learner queue,
     # rest -> actor queue (per-queue CU mask; 96 = 3 XCDs, measured best;
@@ -98,6 +101,13 @@ class Config:
     @property
     def reward_clip_enabled(self) -> bool:
         return self.reward_clip > 0
+
+    @property
+    def fused_model(self) -> bool:
+        """Whether the hand-fused forward kernels compute this model: they
+        have neither the layer norm nor the 8-bit training layer, which run
+        as operators of their own (ops/functional.py)."""
+        return self.fused_forward and not (self.layer_norm or self.fp8_train)
 
     def resolve_device(self) -> str:
         if self.device != "auto":
@@ -161,6 +171,10 @@ def _add_args(p: argparse.ArgumentParser) -> None:
     p.add_argument("--no-fused-forward", dest="fused_forward", action="store_false")
     p.add_argument("--no-fused-backward", dest="fused_backward", action="store_false")
     p.add_argument("--fp8-heads", action="store_true")
+    p.add_argument("--layer-norm", action="store_true",
+                   help="layer norm on the heads' input")
+    p.add_argument("--fp8-train", action="store_true",
+                   help="train the heads' hidden layer on 8-bit blocks")
     p.add_argument("--no-overlap", dest="overlap_colocated", action="store_false")
     p.add_argument("--cu-split", dest="cu_split", type=int, default=d.cu_split)
     p.add_argument("--sharded-replay", action="store_true")

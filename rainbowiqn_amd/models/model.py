@@ -29,6 +29,8 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
+from ..ops.functional import layer_norm, linear_fp8_blocks
+
 CONV_OUT = 3136  # 64 * 7 * 7 for 84x84 input
 
 
@@ -81,6 +83,18 @@ class NoisyLinear(nn.Module):
         self.register_buffer("bias_noisy", self.bias_mu.detach().clone(),
                              persistent=False)
 
+    def effective(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(weight, bias) of this forward pass, differentiable in mu and sigma."""
+        if not self.training:
+            return self.weight_mu, self.bias_mu
+        if getattr(self, "weight_noisy", None) is not None:
+            return (_NoisyValueFn.apply(self.weight_mu, self.weight_sigma,
+                                        self.weight_noisy, self.weight_epsilon),
+                    _NoisyValueFn.apply(self.bias_mu, self.bias_sigma,
+                                        self.bias_noisy, self.bias_epsilon))
+        return (self.weight_mu + self.weight_sigma * self.weight_epsilon,
+                self.bias_mu + self.bias_sigma * self.bias_epsilon)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if self.training:
             if getattr(self, "weight_noisy", None) is not None:
@@ -118,9 +132,42 @@ class _NoisyLinearFn(torch.autograd.Function):
                 None, None, None, None)
 
 
+class _NoisyValueFn(torch.autograd.Function):
+    """The pre-materialized noisy value; backward applies the noise chain rule:
+    dmu = g, dsigma = g * eps."""
+
+    @staticmethod
+    def forward(ctx, mu, sigma, noisy, eps):
+        ctx.save_for_backward(eps)
+        return noisy.view_as(noisy)
+
+    @staticmethod
+    def backward(ctx, g):
+        (eps,) = ctx.saved_tensors
+        return g, g * eps, None, None
+
+
+class LayerNorm(nn.Module):
+    """Layer norm over the last axis (ops.functional.layer_norm)."""
+
+    def __init__(self, features: int, eps: float = 1e-5):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(features))
+        self.bias = nn.Parameter(torch.zeros(features))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+
 class RainbowIQN(nn.Module):
     def __init__(self, cfg, action_space: int):
         super().__init__()
+        use_norm = getattr(cfg, "layer_norm", False)
+        self.fp8_train = getattr(cfg, "fp8_train", False)
+        if (use_norm or self.fp8_train) and getattr(cfg, "fp8_heads", False):
+            raise ValueError("fp8_heads belongs to the fused forward, which has "
+                             "neither layer_norm nor fp8_train")
         self.action_space = action_space
         self.quantile_embedding_dim = cfg.quantile_embedding_dim
         self.history = cfg.history_length
@@ -138,6 +185,7 @@ class RainbowIQN(nn.Module):
         self.fc_h_a = NoisyLinear(self.conv_output_size, cfg.hidden_size, std_init=cfg.noisy_std)
         self.fc_z_v = NoisyLinear(cfg.hidden_size, 1, std_init=cfg.noisy_std)
         self.fc_z_a = NoisyLinear(cfg.hidden_size, action_space, std_init=cfg.noisy_std)
+        self.feature_norm = LayerNorm(self.conv_output_size) if use_norm else None
         # cosine basis multipliers pi * i, i in [0, embedding_dim)
         self.register_buffer(
             "cos_basis",
@@ -168,6 +216,17 @@ class RainbowIQN(nn.Module):
 
     def head(self, h: torch.Tensor) -> torch.Tensor:
         """h: [R, 3136] -> quantile Q values [R, A] (dueling combine)."""
+        if self.feature_norm is not None:
+            h = self.feature_norm(h)
+        if self.fp8_train:
+            # both hidden layers in one product: h is quantised, and kept for
+            # the backward pass, once
+            (wv, bv), (wa, ba) = self.fc_h_v.effective(), self.fc_h_a.effective()
+            hidden = linear_fp8_blocks(h, torch.cat([wv, wa]),
+                                       torch.cat([bv, ba]), relu=True)
+            hv, ha = hidden.chunk(2, dim=1)
+            v, a = self.fc_z_v(hv), self.fc_z_a(ha)
+            return v + a - a.mean(dim=1, keepdim=True)
         v = self.fc_z_v(F.relu(self.fc_h_v(h)))
         a = self.fc_z_a(F.relu(self.fc_h_a(h)))
         return v + a - a.mean(dim=1, keepdim=True)

@@ -70,6 +70,8 @@ class FusedForward:
         self.device = torch.device(device)
         p = net.fc_h_v.weight_mu
         assert p.dtype == torch.bfloat16, "fused forward is the bf16 path"
+        assert net.feature_norm is None and not net.fp8_train, (
+            "fused forward has neither layer norm nor the 8-bit training layer")
         self.A = net.action_space
         d = self.device
         bf = torch.bfloat16

@@ -73,7 +73,7 @@ class GpuActorLoop:
         self.fused = None
         if (self.dtype == torch.bfloat16
                 and net.fc_h_v.weight_mu.dtype == torch.bfloat16
-                and getattr(cfg, "fused_forward", True)):
+                and getattr(cfg, "fused_model", True)):
             from .fused_forward import FusedForward
 
             self.fused = FusedForward.for_net(

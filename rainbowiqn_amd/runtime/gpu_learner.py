@@ -110,7 +110,7 @@ class GpuLearner:
         # hand-written kernels each instead of the eager module stack
         self.fused_online = self.fused_target = None
         self.manual_bwd = False
-        if self.bf16 and getattr(cfg, "fused_forward", True):
+        if self.bf16 and getattr(cfg, "fused_model", True):
             from .fused_forward import FusedForward
 
             fp8 = getattr(cfg, "fp8_heads", False)

@@ -243,7 +243,8 @@ def test_captured_step_replays():
     graphs = []
     for shape in ((256, 3136), (40, 5000)):
         x, w, b, dy = inputs(*shape, torch.bfloat16, torch.bfloat16, "cuda")
-        one = lambda x=x, w=w, b=b, dy=dy: list(step(x, w, b, dy).values())  # noqa: E731
+        one = lambda x=x, w=w, b=b, dy=dy: [  # noqa: E731
+            t.detach() for t in step(x, w, b, dy).values()]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):

@@ -1,0 +1,188 @@
+"""The model with --layer-norm and --fp8-train: layer norm and the 8-bit linear
+layer as the heads use them, one after the other."""
+
+import dataclasses
+
+import pytest
+import torch
+
+from rainbowiqn_amd.config import Config, parse_args
+from rainbowiqn_amd.models import RainbowIQN
+from rainbowiqn_amd.ops import functional as F
+from rainbowiqn_amd.ops import torch_ref
+
+gpu = pytest.mark.gpu
+BOTH = dict(layer_norm=True, fp8_train=True)
+
+
+def test_flags():
+    assert parse_args([]).fused_model
+    cfg = parse_args(["--layer-norm", "--fp8-train"])
+    assert cfg.layer_norm and cfg.fp8_train and not cfg.fused_model
+    assert not parse_args(["--no-fused-forward"]).fused_model
+    with pytest.raises(ValueError):
+        RainbowIQN(parse_args(["--fp8-train", "--fp8-heads"]), 4)
+
+
+def test_off_by_default(cfg):
+    keys = RainbowIQN(cfg, 4).state_dict().keys()
+    assert not any(k.startswith("feature_norm") for k in keys)
+    more = RainbowIQN(dataclasses.replace(cfg, layer_norm=True), 4).state_dict()
+    assert set(more) - set(keys) == {"feature_norm.weight", "feature_norm.bias"}
+
+
+@pytest.mark.parametrize("fused_noise", [False, True])
+def test_noisy_values_have_the_layers_gradients(cfg, fused_noise):
+    torch.manual_seed(0)
+    layer = RainbowIQN(cfg, 4).fc_h_v
+    if fused_noise:
+        layer.enable_fused_noise()
+        with torch.no_grad():
+            layer.weight_noisy.copy_(
+                layer.weight_mu + layer.weight_sigma * layer.weight_epsilon)
+            layer.bias_noisy.copy_(
+                layer.bias_mu + layer.bias_sigma * layer.bias_epsilon)
+    x = torch.randn(5, layer.in_features)
+    grads = []
+    for y in (lambda: layer(x),
+              lambda: torch.nn.functional.linear(x, *layer.effective())):
+        layer.zero_grad()
+        y().sum().backward()
+        grads.append([p.grad.clone() for p in layer.parameters()])
+    for a, b in zip(*grads):
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-5)
+    layer.eval()
+    assert layer.effective()[0] is layer.weight_mu
+
+
+@pytest.mark.parametrize("flags", [dict(layer_norm=True), dict(fp8_train=True), BOTH])
+def test_agent_learns_on_cpu(cfg, flags):
+    from rainbowiqn_amd.agent import Agent
+
+    torch.manual_seed(0)
+    agent = Agent(dataclasses.replace(cfg, **flags), 4, "cpu")
+    b = cfg.batch_size
+    before = {k: p.clone() for k, p in agent.online_net.named_parameters()}
+    loss, per_sample = agent.learn_from_batch(
+        torch.rand(b, 4, 84, 84), torch.randint(0, 4, (b,)), torch.randn(b),
+        torch.rand(b, 4, 84, 84), torch.ones(b), torch.ones(b))
+    assert torch.isfinite(loss) and per_sample.shape == (b,)
+    for k, p in agent.online_net.named_parameters():
+        assert torch.isfinite(p).all()
+        assert not torch.equal(p, before[k]), k
+    assert agent.act(torch.rand(4, 84, 84)) in range(4)
+
+
+def check_head(net, h, device):
+    """head() forward and backward, stage by stage from its own intermediate
+    results, against 64-bit forms.  A result is rounded by half a step, eps / 2
+    of its value, and eps leaves as much for its fp32 sums; 8-bit products lose
+    less than 7 x 2^-13 of their magnitude (tests/test_fp8_blocks.py)."""
+    seen = {}
+    real_norm, real_linear = F.layer_norm, F.linear_fp8_blocks
+
+    def norm(x, w, b, eps):
+        seen["norm"] = real_norm(x, w, b, eps)
+        seen["norm"].retain_grad()
+        return seen["norm"]
+
+    def linear(x, w, b, relu):
+        seen["w"], seen["b"] = w.detach(), b.detach()
+        seen["hidden"] = real_linear(x, w, b, relu=relu)
+        seen["hidden"].retain_grad()
+        return seen["hidden"]
+
+    from rainbowiqn_amd.models import model
+
+    model.layer_norm, model.linear_fp8_blocks = norm, linear
+    try:
+        q = net.head(h)
+    finally:
+        model.layer_norm, model.linear_fp8_blocks = real_norm, real_linear
+    q.float().square().sum().backward()
+    d = lambda t: t.detach().double().cpu()  # noqa: E731
+    held = lambda t, r: torch_ref.dequantize_fp8_blocks(  # noqa: E731
+        *torch_ref.quantize_fp8_blocks(t.detach().float().cpu(), r), t.shape[1],
+        r).double()
+    # forward: norm, then the hidden layers
+    x = d(h)
+    std = (x.var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+    n = (x - x.mean(1, keepdim=True)) / std
+    fn = net.feature_norm
+    eps = torch.finfo(h.dtype).eps
+    close(seen["norm"], n * d(fn.weight) + d(fn.bias), eps)
+    xh, wh = held(seen["norm"], 1), held(seen["w"], 128)
+    z = (xh @ wh.t() + d(seen["b"])).clamp(min=0)
+    lost = 7 * 2.0 ** -13 * (xh.abs() @ wh.abs().t())
+    close(seen["hidden"], z, eps, lost)
+    # backward: hidden layers, then norm
+    dz = d(seen["hidden"].grad) * (d(seen["hidden"]) > 0)
+    g = held(dz.float(), 1)
+    close(seen["norm"].grad, g @ wh, eps, 7 * 2.0 ** -13 * (g.abs() @ wh.abs()))
+    dw = g.t() @ xh
+    close(net.fc_h_v.weight_mu.grad, dw[:512], eps)
+    close(net.fc_h_a.weight_sigma.grad,
+          dw[512:] * d(net.fc_h_a.weight_epsilon), 2 * eps)
+    close(net.fc_h_v.bias_mu.grad, dz.sum(0)[:512], eps)
+    dy = d(seen["norm"].grad)
+    gw = dy * d(fn.weight)
+    dx = (gw - gw.mean(1, keepdim=True) - n * (gw * n).mean(1, keepdim=True)) / std
+    close(h.grad, dx, eps)
+    close(fn.weight.grad, (dy * n).sum(0), eps)
+    close(fn.bias.grad, dy.sum(0), eps)
+
+
+def close(got, want, eps, more=0.0):
+    # sums of up to 3136 terms in fp32 beside the rounding of the result
+    bound = eps * want.abs() + 2.0 ** -18 * want.abs().max() + more
+    off = (got.detach().double().cpu() - want).abs() - bound
+    assert bool((off <= 0).all()), float(off.max())
+
+
+def head_and_input(device, dtype, rows):
+    torch.manual_seed(1)
+    net = RainbowIQN(Config(hidden_size=512, **BOTH), 6).to(device).to(dtype).train()
+    with torch.no_grad():
+        net.feature_norm.weight.add_(0.1 * torch.randn(3136, device=device).to(dtype))
+        net.feature_norm.bias.add_(0.1 * torch.randn(3136, device=device).to(dtype))
+    h = (torch.rand(rows, 3136) * torch.rand(rows, 1)).to(dtype).to(device)
+    return net, h.requires_grad_()
+
+
+def test_head_cpu():
+    net, h = head_and_input("cpu", torch.float32, 20)
+    check_head(net, h, "cpu")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 33, 256, 2000])
+def test_head_gpu(rows, dtype):
+    net, h = head_and_input("cuda", dtype, rows)
+    check_head(net, h, "cuda")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("flags", [dict(layer_norm=True), dict(fp8_train=True), BOTH])
+def test_learner_and_actor(flags, dtype):
+    """Captured rounds of actor and learner run, losses stay finite and every
+    parameter moves."""
+    from rainbowiqn_amd.parallel.apex import ApexRunner
+    from rainbowiqn_amd.parallel.comm import Communicator
+
+    cfg = Config(device="cuda", dtype=dtype, learn_start=256, memory_capacity=8192,
+                 learn_per_round=2, cu_split=0, **flags)
+    runner = ApexRunner(cfg, Communicator(backend="auto"), n_envs=32, chunk_steps=8)
+    assert runner.fast and runner.glearner.fused_online is None
+    before = runner.glearner.master_flat.clone()
+    for _ in range(5):
+        runner.run_round()
+    torch.cuda.synchronize()
+    assert runner.grad_steps > 0 and runner.glearner.graph is not None
+    assert all(torch.isfinite(torch.tensor(l)) for l in runner.losses)
+    after = runner.glearner.master_flat
+    assert torch.isfinite(after).all() and not torch.equal(after, before)
+    for k, p in runner.glearner.online.named_parameters():
+        if k.startswith(("feature_norm", "fc_h")):
+            assert p.grad.any(), k
