@@ -967,6 +967,8 @@ __global__ __launch_bounds__(256, 2) void wgrad_kernel(Wgrad w) {
     const int og = rg * (int)ldg + bn * 128 + (there ? pg : pg & 7) * 16;
     const int os = rg * w.Sn + bn + (there ? pg >> 3 : 0);
     const int ox = rx * (int)ldx + bk * 128 + px * 16, ot = rx * w.Sk + bk;
+    // rows behind the last one are told by the lane's own offset alone
+    const int og2[2] = {og, og + 16 * (int)ldg}, os2[2] = {os, os + 16 * w.Sn};
     struct Held { i32x4 v[3]; int e[3]; };
     auto load = [&](Held& h, int step) {
         const int64_t m = lo + (int64_t)step * 32;
@@ -977,9 +979,8 @@ __global__ __launch_bounds__(256, 2) void wgrad_kernel(Wgrad w) {
         const auto bt = buffer_of(w.xs + m * w.Sk, left * w.Sk);
         #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            h.v[i] = __builtin_amdgcn_raw_buffer_load_b128(
-                bg, og, i * 16 * (int)ldg, 0);
-            h.e[i] = __builtin_amdgcn_raw_buffer_load_b8(bs, os, i * 16 * w.Sn, 0);
+            h.v[i] = __builtin_amdgcn_raw_buffer_load_b128(bg, og2[i], 0, 0);
+            h.e[i] = __builtin_amdgcn_raw_buffer_load_b8(bs, os2[i], 0, 0);
         }
         h.v[2] = __builtin_amdgcn_raw_buffer_load_b128(bx, ox, 0, 0);
         h.e[2] = __builtin_amdgcn_raw_buffer_load_b8(bt, ot, 0, 0);
