@@ -236,6 +236,12 @@ std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
     return s;
 }
 
+// y in another shape, but no view of y: a view that a custom function returns
+// refuses to be changed in place
+Tensor shaped(const Tensor& y, c10::IntArrayRef shape) {
+    return y.sizes() == shape ? y : at::_unsafe_view(y, shape);
+}
+
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t && t->requires_grad(); }
 
@@ -249,6 +255,28 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads) {
     auto err = std::make_shared<torch::autograd::DelayedError>(
         "this operator is differentiable once", (int)fake.size());
     return (*err)(std::move(fake));
+}
+
+// A gradient that goes on to a node of the default stream, such as a leaf's that
+// a graph built outside the capture keeps alive, cannot be captured: the wait
+// between the streams would break the capture and end the process.
+void check_capture(const Tensor& t) {
+    const auto stream = at::cuda::getCurrentCUDAStream(t.device().index());
+    const c10::Stream other =
+        at::cuda::getDefaultCUDAStream(t.device().index()).unwrap();
+    if (stream.unwrap() == other) return;
+    hipStreamCaptureStatus status;
+    const hipError_t err = hipStreamIsCapturing(stream.stream(), &status);
+    TORCH_CHECK(err == hipSuccess, hipGetErrorString(err));
+    const auto node = torch::autograd::get_current_node();
+    if (status == hipStreamCaptureStatusNone || !node) return;
+    for (const auto& e : node->next_edges()) {
+        if (!e.function) continue;
+        const auto s = e.function->stream();
+        TORCH_CHECK(!s || *s != other,
+                    "a backward pass cannot be captured while a graph built on "
+                    "the default stream is alive: drop its results first");
+    }
 }
 
 struct LinearSaved {
@@ -379,11 +407,12 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
         d["dx"] = ndx ? (int64_t)x.scalar_type() : -1;
         d["dw"] = ndw ? (int64_t)w.scalar_type() : -1;
         d["db"] = ndb ? (int64_t)bias->scalar_type() : -1;
-        return y.view(with_last(x, w.size(0)));
+        return shaped(y, with_last(x, w.size(0)));
     }
     static torch::autograd::variable_list backward(
         torch::autograd::AutogradContext* ctx,
         torch::autograd::variable_list dy) {
+        check_capture(dy[0]);
         const auto v = ctx->get_saved_variables();
         auto& d = ctx->saved_data;
         const auto shape = d["shape"].toIntVector();
@@ -395,7 +424,7 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
         LinearGrads g = linear_bwd(as_rows(dy[0]), {v[0], v[1], v[2], v[3], v[4]},
                                    shape.back(), type("dx"), type("dw"),
                                    type("db"));
-        if (g.dx.defined()) g.dx = g.dx.view(shape);
+        if (g.dx.defined()) g.dx = shaped(g.dx, shape);
         return once({g.dx, g.dw, g.db, Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
@@ -404,8 +433,9 @@ Tensor linear_fp8(Tensor x, Tensor w, OptTensor bias, bool relu) {
     TORCH_CHECK(w.dim() == 2, "weight must have 2 dimensions");
     if (!at::GradMode::is_enabled() ||
         !(wants_grad(x) || wants_grad(w) || wants_grad(bias)))
-        return linear_fwd(as_rows(x), as_rows(w), bias, relu, false, nullptr)
-            .view(with_last(x, w.size(0)));
+        return shaped(
+            linear_fwd(as_rows(x), as_rows(w), bias, relu, false, nullptr),
+            with_last(x, w.size(0)));
     return LinearFn::apply(x, w, bias, relu, wants_grad(x), wants_grad(w),
                            wants_grad(bias));
 }
@@ -440,7 +470,7 @@ Tensor linear_fp8_serve(Tensor x0, Tensor wq, Tensor ws, int64_t block_rows,
     else if (y.numel() > 0)
         gemm(quant_rows(x, nullptr, nullptr), w, x.size(1), bias, relu, y,
              nullptr);
-    return y.view(with_last(x0, w.rows));
+    return shaped(y, with_last(x0, w.rows));
 }
 
 int norm_weights(const Tensor& x, const OptTensor& w, const OptTensor& b) {
@@ -495,11 +525,12 @@ class NormFn : public torch::autograd::Function<NormFn> {
         d["shape"] = x.sizes().vec();
         d["wtype"] = (int64_t)(w ? *w : b ? *b : x).scalar_type();
         d["need"] = (int64_t)(ndx | ndw << 1 | ndb << 2);
-        return y.view(x.sizes());
+        return shaped(y, x.sizes());
     }
     static torch::autograd::variable_list backward(
         torch::autograd::AutogradContext* ctx,
         torch::autograd::variable_list grad) {
+        check_capture(grad[0]);
         const auto v = ctx->get_saved_variables();
         const Tensor &x = v[0], &w = v[1], &mean = v[2], &rstd = v[3];
         auto& d = ctx->saved_data;
@@ -535,7 +566,7 @@ class NormFn : public torch::autograd::Function<NormFn> {
                          (int)R, (int)C, stream_of(x)),
                      "layer_norm backward");
         }
-        if (need & 1) dx = dx.view(d["shape"].toIntVector());
+        if (need & 1) dx = shaped(dx, d["shape"].toIntVector());
         return once({dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
@@ -543,8 +574,8 @@ class NormFn : public torch::autograd::Function<NormFn> {
 Tensor layer_norm(Tensor x, OptTensor w, OptTensor b, double eps) {
     if (!at::GradMode::is_enabled() ||
         !(wants_grad(x) || wants_grad(w) || wants_grad(b)))
-        return norm_fwd(as_rows(x), w, b, eps, nullptr, nullptr)
-            .view(x.sizes());
+        return shaped(norm_fwd(as_rows(x), w, b, eps, nullptr, nullptr),
+                      x.sizes());
     return NormFn::apply(x, w, b, eps, wants_grad(x), wants_grad(w),
                          wants_grad(b));
 }

@@ -183,7 +183,8 @@ class _LinearFp8CpuFn(torch.autograd.Function):
         ctx.shape = x.shape
         ctx.dtypes = (x.dtype, weight.dtype,
                       None if bias is None else bias.dtype)
-        return y.view(*x.shape[:-1], weight.shape[0])
+        # no view: that could not be changed in place
+        return torch.ops.aten._unsafe_view(y, [*x.shape[:-1], weight.shape[0]])
 
     @staticmethod
     @once_differentiable

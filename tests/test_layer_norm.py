@@ -281,3 +281,45 @@ def test_offsets_past_32_bits():
     for name in got:
         near(got[name], *want[name])
     assert not dx[:-50].any()
+
+
+def changed_in_place(device):
+    """A result may be changed in place, like any other."""
+    x = torch.randn(6, 40, device=device, requires_grad=True)
+    w = torch.randn(40, device=device, requires_grad=True)
+    for shape in ((6, 40), (2, 3, 40)):
+        want = torch.relu(F.layer_norm(x.view(shape), w) * 2)
+        got = F.layer_norm(x.view(shape), w).mul_(2).relu_()
+        assert torch.equal(got, want)
+        for p, q in zip(torch.autograd.grad(got.sum(), (x, w)),
+                        torch.autograd.grad(want.sum(), (x, w))):
+            assert torch.equal(p, q)
+
+
+def test_changed_in_place_cpu():
+    changed_in_place("cpu")
+
+
+@gpu
+def test_changed_in_place_gpu():
+    changed_in_place("cuda")
+
+
+@gpu
+def test_capture_beside_an_eager_graph_is_refused():
+    x = torch.randn(6, 200, device="cuda", requires_grad=True)
+    w = torch.randn(200, device="cuda", requires_grad=True)
+    call = lambda: F.layer_norm(x, w)  # noqa: E731
+    alive = call()  # holds the leaves' nodes, which are of the default stream
+    dy = torch.ones_like(alive)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call()
+        with pytest.raises(RuntimeError, match="captured"):
+            torch.autograd.grad(y, (x, w), dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, alive)
+    alive.backward(dy)  # that one is as before
+    assert x.grad.shape == x.shape
