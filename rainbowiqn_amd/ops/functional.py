@@ -210,6 +210,9 @@ def linear_fp8_blocks(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = No
         dx = g Q(W)    dW = g^T Q(x)    db = sum of dz's rows
     that is, rounding to 8 bits counts as the identity."""
     if isinstance(weight, Fp8Blocks):
+        if x.dim() > 0 and x.shape[-1] != weight.cols:
+            raise RuntimeError(f"x has {x.shape[-1]} columns and weight "
+                               f"{weight.cols}")
         if x.is_cuda:
             return get_extension().linear_fp8_serve(
                 x, weight.q, weight.scale, weight.block_rows, bias, relu)

@@ -546,3 +546,130 @@ def test_capture_beside_an_eager_graph_is_refused():
     assert torch.equal(y, alive)
     alive.backward(dy)  # that one is as before
     assert x.grad.shape == x.shape
+
+
+def served_columns(device):
+    """A weight of other columns is refused also where its blocks are as many."""
+    w = F.quantize_fp8_blocks(torch.randn(8, 200, device=device), 128)
+    for cols in (199, 201, 256):
+        with pytest.raises(RuntimeError, match="columns"):
+            F.linear_fp8_blocks(torch.randn(4, cols, device=device), w)
+    with pytest.raises(RuntimeError):
+        F.linear_fp8_blocks(torch.tensor(1.0, device=device), w)
+
+
+def test_served_columns_cpu():
+    served_columns("cpu")
+
+
+@gpu
+def test_served_columns_gpu():
+    served_columns("cuda")
+
+
+@gpu
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [
+    (1, 1, 1), (1, 17, 5000), (2, 15, 127), (3, 1000, 136), (7, 33, 1023),
+    (15, 16, 128), (16, 100, 3968), (16, 100, 4096), (16, 40, 5000),
+    (8, 70, 8000), (17, 40, 300), (1, 20, 60000), (1, 20, 70000)])
+def test_serving_a_few_rows(m, n, k, dtype, relu):
+    """On both sides of 16 rows and of what fits into local memory; rows that
+    begin anywhere."""
+    wide = (0.25 * matrix(m, k + 3, 1)).clamp(-8, 8).to(dtype).cuda()
+    w = torch.rand(n, k, generator=torch.Generator().manual_seed(2)) - 0.5
+    b = matrix(1, n, 3)[0].clamp(-1, 1).cuda()
+    for block_rows in (1, 128):
+        wb = F.quantize_fp8_blocks(w.cuda(), block_rows)
+        for x in (wide[:, :k].contiguous(), wide[:, 3:]):
+            z = held(x) @ held(w, block_rows).t() + b.double().cpu()
+            size = (held(x).abs() @ held(w, block_rows).abs().t()
+                    + b.double().cpu().abs())
+            y = F.linear_fp8_blocks(x, wb, b, relu)
+            near(y, z.clamp(min=0) if relu else z, tol(k + 1, size, z, dtype))
+
+
+@gpu
+def test_serving_takes_what_is_not_finite():
+    x = torch.randn(5, 300, device="cuda")
+    x[1, 200], x[3, 7] = float("inf"), float("nan")
+    w = F.quantize_fp8_blocks(torch.randn(40, 300, device="cuda"), 128)
+    y = F.linear_fp8_blocks(x, w)
+    assert y[[1, 3]].isnan().all() and y[[0, 2, 4]].isfinite().all()
+    ok = F.linear_fp8_blocks(x[[0, 2, 4]], w)
+    assert torch.equal(y[[0, 2, 4]], ok)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 12, 400])
+def test_captured_serving_replays(m):
+    x = matrix(m, 500, 1, torch.bfloat16, "cuda")
+    w = F.quantize_fp8_blocks(matrix(300, 500, 2, device="cuda"), 128)
+    one = lambda: F.linear_fp8_blocks(x, w, relu=True)  # noqa: E731
+    one()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = one()
+    for i in range(4):
+        x.copy_(matrix(m, 500, 10 + i, torch.bfloat16, "cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, one())
+
+
+@gpu
+@pytest.mark.parametrize("dtypes", [(torch.float32, torch.bfloat16),
+                                    (torch.float16, torch.float32)])
+@pytest.mark.parametrize("m,n,k,at", [(300, 200, 520, 0), (40, 130, 264, 3),
+                                      (7, 500, 128, 1), (2000, 64, 96, 0)])
+def test_linear_of_two_types_and_any_start(m, n, k, at, dtypes):
+    """Activation and weight of two types, or beginning anywhere, are held in 8
+    bits as each is by itself."""
+    x = (0.25 * matrix(m, k + at, 1)).clamp(-8, 8).to(dtypes[0]).cuda()[:, at:]
+    w = matrix(n, k + at, 2).clamp(-4, 4).to(dtypes[1]).cuda()[:, at:]
+    x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+    dy = (0.1 * matrix(m, n, 4)).clamp(-2, 2).to(dtypes[0]).cuda()
+    y = F.linear_fp8_blocks(x, w, relu=True)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    check_linear(x, w, None, dy, y, dx, dw, None, True)
+
+
+@gpu
+def test_two_calls_at_once():
+    """On two streams, each with its own workspaces."""
+    args = [(matrix(m, k, 1, torch.bfloat16, "cuda").requires_grad_(),
+             matrix(n, k, 2, torch.bfloat16, "cuda").requires_grad_(),
+             matrix(m, n, 4, torch.bfloat16, "cuda"))
+            for m, n, k in ((3000, 300, 500), (2000, 400, 700))]
+
+    def one(x, w, dy):
+        return torch.autograd.grad(F.linear_fp8_blocks(x, w, relu=True), (x, w), dy)
+
+    want = [one(*a) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    got = [None, None]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got[i] = one(*args[i])
+        torch.cuda.synchronize()
+        for p, q in zip(got, want):
+            assert all(torch.equal(a, b) for a, b in zip(p, q))
+
+
+@gpu
+def test_the_same_tensor_twice():
+    x = matrix(130, 130, 1, device="cuda").requires_grad_()
+    dy = matrix(130, 130, 2, device="cuda")
+    a, b = x.detach().clone().requires_grad_(), x.detach().clone().requires_grad_()
+    (g,) = torch.autograd.grad(F.linear_fp8_blocks(x, x), x, dy)
+    p, q = torch.autograd.grad(F.linear_fp8_blocks(a, b), (a, b), dy)
+    assert torch.equal(g, p + q)
+    blocks = F.quantize_fp8_blocks(x)
+    twin = blocks._replace(q=blocks.q.clone(), scale=blocks.scale.clone())
+    assert torch.equal(F.matmul_fp8_blocks(blocks, blocks),
+                       F.matmul_fp8_blocks(blocks, twin))
