@@ -305,7 +305,8 @@ __global__ __launch_bounds__(256, 2) void norm_bwd_kernel(NormBwd a) {
     float dw[NV][8], db[NV][8];
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        w[i] = a.w ? load8<W, VEC, false>((const W*)a.w, (i * 64 * TW + t) * 8, a.C)
+        // zeros behind column C: an infinite weight times dy's zeros were NaN
+        w[i] = a.w ? load8<W, VEC, true>((const W*)a.w, (i * 64 * TW + t) * 8, a.C)
                    : all8<W>(1.0f);
         #pragma unroll
         for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.0f;
@@ -427,20 +428,21 @@ __global__ __launch_bounds__(256) void norm_dx_long_kernel(NormBwd a) {
     }
 }
 
-// a column a thread, a share of the rows a workgroup
+// a column a thread, a share of the rows a workgroup; columns along x, of which
+// a grid may have more than along y
 template <typename T>
 __global__ __launch_bounds__(256) void norm_part_long_kernel(NormBwd a) {
-    const int c = blockIdx.y * 256 + threadIdx.x;
+    const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= a.C) return;
     float dw = 0.0f, db = 0.0f;
-    for (int64_t r = blockIdx.x; r < a.R; r += gridDim.x) {
+    for (int64_t r = blockIdx.y; r < a.R; r += gridDim.y) {
         const float d = to_f(((const T*)a.dy)[r * a.lddy + c]);
         const float h =
             (to_f(((const T*)a.x)[r * a.ldx + c]) - a.mean[r]) * a.rstd[r];
         dw += d * h;
         db += d;
     }
-    float* part = a.part + (int64_t)blockIdx.x * 2 * a.C;
+    float* part = a.part + (int64_t)blockIdx.y * 2 * a.C;
     part[c] = dw;
     part[a.C + c] = db;
 }
@@ -550,7 +552,7 @@ int riqn_norm_bwd(const void* dy, const void* x, int type, int64_t lddy,
                                    dim3(min(R, 1 << 16)), dim3(256), 0, st, a);
             if (part)
                 hipLaunchKernelGGL((norm_part_long_kernel<T>),
-                                   dim3(groups, (C + 255) / 256), dim3(256), 0,
+                                   dim3((C + 255) / 256, groups), dim3(256), 0,
                                    st, a);
         } else {
             RIQN_NORM_SHAPE(C, {

@@ -323,3 +323,44 @@ def test_capture_beside_an_eager_graph_is_refused():
     assert torch.equal(y, alive)
     alive.backward(dy)  # that one is as before
     assert x.grad.shape == x.shape
+
+
+@gpu
+def test_most_columns():
+    x = torch.randn(2, 2 ** 24, device="cuda").bfloat16().requires_grad_()
+    w = torch.rand(2 ** 24, device="cuda").requires_grad_()
+    dy = torch.randn(2, 2 ** 24, device="cuda").bfloat16()
+    F.layer_norm(x, w).backward(dy)
+    h = x.detach().double()
+    h = h - h.mean(1, keepdim=True)
+    h = h / (h.pow(2).mean(1, keepdim=True) + 1e-5).sqrt()
+    # sums of 2^24 terms of either sign in fp32, by 256 threads of 2^16 each,
+    # leave mean and rstd 2^16 x 2^-24 of a term off at the very most
+    want = (dy.double() * h).sum(0)
+    off = (w.grad.double() - want).abs()
+    assert bool((off <= 2.0 ** -7 * (dy.double() * h).abs().sum(0) + 2.0 ** -7
+                 * dy.double().abs().sum(0)).all())
+    with pytest.raises(RuntimeError):
+        F.layer_norm(torch.empty(1, 2 ** 24 + 1, device="cuda"))
+
+
+@gpu
+@pytest.mark.parametrize("cols", [8, 520, 1001, 1040, 2056, 4104])
+def test_infinite_weight_stays_in_its_column(cols):
+    """y and dw of the others are finite.  Both means of dx are infinite, mean(g)
+    with the sign of dy there and mean(g h) with h's as well, so
+    g - mean(g) - h mean(g h) is infinite where h has the sign of that column's
+    and NaN where it has the other."""
+    x = torch.randn(5, cols, device="cuda", requires_grad=True)
+    w = torch.ones(cols, device="cuda")
+    w[-1] = float("inf")
+    w.requires_grad_()
+    dy = torch.randn(5, cols, device="cuda")
+    y = F.layer_norm(x, w)
+    assert y[:, :-1].isfinite().all() and y[:, -1].isinf().all()
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert dw.isfinite().all()
+    h = x - x.mean(1, keepdim=True)
+    same = (h * h[:, -1:] > 0)[:, :-1]
+    assert torch.equal(dx[:, :-1].isnan(), ~same)
+    assert dx[:, :-1][same].isinf().all()
