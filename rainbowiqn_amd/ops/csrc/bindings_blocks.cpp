@@ -56,9 +56,19 @@ void check_vector(const Tensor& v, int64_t n, const Tensor& like,
 int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
 int64_t padded4(int64_t n) { return (n + 3) / 4 * 4; }
 
+// a matrix in 8-bit blocks where it lies; the memory is another's
+struct Mat {
+    uint8_t *q, *scale;
+    int64_t rows, block_rows;
+};
+
 struct Blocks {
     Tensor q, scale;
     int64_t rows, block_rows;
+    Mat mat() const {
+        return {q.data_ptr<uint8_t>(), scale.data_ptr<uint8_t>(), rows,
+                block_rows};
+    }
 };
 
 // checks what the kernels take for granted about a matrix given from outside
@@ -117,29 +127,51 @@ int quant_groups(int64_t R, int64_t C, int64_t most) {
     return row_groups(R, blocks_of(C) >= 4 ? 4 : 16, most);
 }
 
+// Parts of one allocation: a training step of few rows is bound by the host,
+// which each allocation costs 1.4 us and each tensor saved for the backward pass
+// about as much.  [256, 1024, 3136]: 82 us a step, with 10 more of them 96.
+struct Carve {
+    int64_t size = 0;
+    int64_t take(int64_t bytes) {
+        const int64_t at = size;
+        size += (bytes + 255) / 256 * 256;
+        return at;
+    }
+    // a matrix [R, C]: where its bytes and its scales begin
+    std::pair<int64_t, int64_t> matrix(int64_t R, int64_t C,
+                                       int64_t block_rows) {
+        const int64_t nb = blocks_of(C), q = take(R * nb * 128);
+        return {q, take((block_rows == 1 ? R : blocks_of(R)) * padded4(nb))};
+    }
+};
+
+Mat mat_at(uint8_t* base, std::pair<int64_t, int64_t> at, int64_t rows,
+           int64_t block_rows) {
+    return {base + at.first, base + at.second, rows, block_rows};
+}
+
+// Groups of rows for a quantisation that also sums up the columns: every group
+// leaves a row of partial sums to be added up, and 1024 workgroups in all fill
+// the card and keep those few.
+int sum_groups(int64_t R, int64_t C) {
+    const int64_t nb = blocks_of(C), strips = nb >= 4 ? (nb + 3) / 4 : nb;
+    return quant_groups(R, C, std::max<int64_t>(1, 1024 / strips));
+}
+
 // scale per 1 x 128 block; with `mask` values whose bit is clear count as
-// zero; `sum` (may be null) gets the sums of the columns
-Blocks quant_rows(const Tensor& x, const uint8_t* mask, Tensor* sum) {
-    const int64_t R = x.size(0), C = x.size(1), nb = blocks_of(C);
-    Blocks o = new_blocks(x, R, C, 1);
-    // with sums every group leaves a row of partial ones to be added up: 1024
-    // workgroups in all fill the card and keep those few
-    const int64_t strips = nb >= 4 ? (nb + 3) / 4 : nb;
-    const int groups = quant_groups(
-        R, C, sum ? std::max<int64_t>(1, 1024 / strips) : 65535);
-    Tensor part;
-    if (sum) part = torch::empty({groups, C}, floats_on(x));
-    launched(riqn_fp8_quant_rows(
-                 x.data_ptr(), type_code(x.scalar_type(), "x"), x.stride(0),
-                 mask, o.q.data_ptr<uint8_t>(), o.scale.data_ptr<uint8_t>(),
-                 sum ? part.data_ptr<float>() : nullptr, groups, (int)R,
-                 (int)C, stream_of(x)),
+// zero; `part` (may be null, [groups, C]) gets sums of the columns
+void quant_rows(const Tensor& x, const uint8_t* mask, const Mat& o, float* part,
+                int groups) {
+    launched(riqn_fp8_quant_rows(x.data_ptr(),
+                                 type_code(x.scalar_type(), "x"), x.stride(0),
+                                 mask, o.q, o.scale, part, groups,
+                                 (int)x.size(0), (int)x.size(1), stream_of(x)),
              "quantize_fp8_blocks");
-    if (sum)
-        launched(riqn_column_sum(part.data_ptr<float>(), sum->data_ptr(),
-                                 type_code(sum->scalar_type(), "bias"), groups,
-                                 (int)C, stream_of(x)),
-                 "column sum");
+}
+Blocks quant_rows(const Tensor& x) {
+    Blocks o = new_blocks(x, x.size(0), x.size(1), 1);
+    quant_rows(x, nullptr, o.mat(), nullptr,
+               quant_groups(x.size(0), x.size(1), 65535));
     return o;
 }
 
@@ -162,13 +194,11 @@ Blocks quant_tiles(const Tensor& x) {
     return o;
 }
 
-void gemm(const Blocks& a, const Blocks& b, int64_t K, const OptTensor& bias,
+void gemm(const Mat& a, const Mat& b, int64_t K, const OptTensor& bias,
           bool relu, Tensor& c, uint8_t* mask) {
     launched(riqn_fp8_gemm(
-                 a.q.data_ptr<uint8_t>(), a.scale.data_ptr<uint8_t>(),
-                 (int)a.block_rows, b.q.data_ptr<uint8_t>(),
-                 b.scale.data_ptr<uint8_t>(), (int)b.block_rows,
-                 bias ? bias->data_ptr() : nullptr,
+                 a.q, a.scale, (int)a.block_rows, b.q, b.scale,
+                 (int)b.block_rows, bias ? bias->data_ptr() : nullptr,
                  bias ? type_code(bias->scalar_type(), "bias") : 0, relu,
                  c.data_ptr(), type_code(c.scalar_type(), "out"), mask,
                  (int)a.rows, (int)b.rows, (int)K, stream_of(c)),
@@ -182,7 +212,7 @@ std::tuple<Tensor, Tensor> fp8_blocks_quant(Tensor x, int64_t block_rows) {
     type_code(x.scalar_type(), "x");
     c10::cuda::CUDAGuard guard(x.device());
     Blocks o = x.size(0) == 0    ? new_blocks(x, 0, x.size(1), block_rows)
-               : block_rows == 1 ? quant_rows(x, nullptr, nullptr)
+               : block_rows == 1 ? quant_rows(x)
                                  : quant_tiles(x);
     return {o.q, o.scale};
 }
@@ -215,7 +245,7 @@ Tensor fp8_blocks_matmul(Tensor aq, Tensor as, int64_t a_block_rows, Tensor bq,
     c10::cuda::CUDAGuard guard(aq.device());
     Tensor c = torch::empty({a.rows, b.rows}, aq.options().dtype(dtype));
     if (c.numel() == 0) return c;
-    gemm(a, b, cols, bias, relu, c, nullptr);
+    gemm(a.mat(), b.mat(), cols, bias, relu, c, nullptr);
     return c;
 }
 
@@ -279,15 +309,23 @@ void check_capture(const Tensor& t) {
     }
 }
 
-struct LinearSaved {
-    Tensor xq, xs;                // x in 8 bits
-    Tensor wtq, wts;              // W transposed in 8 bits, for dx
-    Tensor bits;                  // the relu's
+// What waits for the backward pass, in one allocation: x in 8 bits; W
+// transposed in 8 bits, for dx; the relu's bits.
+struct Kept {
+    std::pair<int64_t, int64_t> x, wt;
+    int64_t bits, size;
+    Kept(int64_t M, int64_t N, int64_t K, bool dx, bool relu) {
+        Carve c;
+        x = c.matrix(M, K, 1);
+        if (dx) wt = c.matrix(K, N, 128);
+        bits = c.take(relu ? M * blocks_of(N) * 16 : 0);
+        size = c.size;
+    }
 };
 
-// y = x W^T + bias, relu; `keep` gets what the backward pass reads
+// y = x W^T + bias, relu; `keep` gets what the backward pass reads (Kept)
 Tensor linear_fwd(const Tensor& x, const Tensor& w, const OptTensor& bias,
-                  bool relu, bool need_dx, LinearSaved* keep) {
+                  bool relu, bool need_dx, Tensor* keep) {
     check_rows(x, "x");
     check_rows(w, "weight");
     TORCH_CHECK(w.device() == x.device(), "weight must be on ", x.device());
@@ -305,40 +343,32 @@ Tensor linear_fwd(const Tensor& x, const Tensor& w, const OptTensor& bias,
     const int64_t M = x.size(0), N = w.size(0), K = x.size(1);
     Tensor y = torch::empty({M, N}, x.options());
     if (M == 0 && !keep) return y;
-    Blocks xq = new_blocks(x, M, K, 1), wq = new_blocks(x, N, K, 128), wt;
-    uint8_t *wtq = nullptr, *wts = nullptr;
-    if (need_dx) {
-        wt = new_blocks(x, K, N, 128);
-        wtq = wt.q.data_ptr<uint8_t>();
-        wts = wt.scale.data_ptr<uint8_t>();
-    }
-    auto *xp = xq.q.data_ptr<uint8_t>(), *xsp = xq.scale.data_ptr<uint8_t>();
-    auto *wp = wq.q.data_ptr<uint8_t>(), *wsp = wq.scale.data_ptr<uint8_t>();
+    const Kept at(M, N, K, need_dx, relu && keep);
+    Carve c;
+    const auto w_at = c.matrix(N, K, 128);
+    const int64_t x_at = c.take(keep ? 0 : at.size);
+    Tensor work = torch::empty({c.size}, bytes_on(x));
+    auto* const base = work.data_ptr<uint8_t>();
+    if (keep) *keep = torch::empty({at.size}, bytes_on(x));
+    auto* const kept = keep ? keep->data_ptr<uint8_t>() : base + x_at;
+    const Mat xq = mat_at(kept, at.x, M, 1), wq = mat_at(base, w_at, N, 128);
+    const Mat wt = need_dx ? mat_at(kept, at.wt, K, 128) : Mat{};
     const int groups = quant_groups(M, K, 65535);
     if (M > 0 && type == w_type) {
-        launched(riqn_fp8_quant_both(x.data_ptr(), x.stride(0), xp, xsp, groups,
-                                     (int)M, w.data_ptr(), w.stride(0), wp, wsp,
-                                     wtq, wts, (int)N, (int)K, type,
-                                     stream_of(x)),
+        launched(riqn_fp8_quant_both(x.data_ptr(), x.stride(0), xq.q, xq.scale,
+                                     groups, (int)M, w.data_ptr(), w.stride(0),
+                                     wq.q, wq.scale, wt.q, wt.scale, (int)N,
+                                     (int)K, type, stream_of(x)),
                  "linear_fp8_blocks");
     } else {
-        if (M > 0)
-            launched(riqn_fp8_quant_rows(x.data_ptr(), type, x.stride(0),
-                                         nullptr, xp, xsp, nullptr, groups,
-                                         (int)M, (int)K, stream_of(x)),
-                     "linear_fp8_blocks");
-        launched(riqn_fp8_quant_tiles(w.data_ptr(), w_type, w.stride(0), wp,
-                                      wsp, wtq, wts, (int)N, (int)K,
+        if (M > 0) quant_rows(x, nullptr, xq, nullptr, groups);
+        launched(riqn_fp8_quant_tiles(w.data_ptr(), w_type, w.stride(0), wq.q,
+                                      wq.scale, wt.q, wt.scale, (int)N, (int)K,
                                       stream_of(x)),
                  "linear_fp8_blocks");
     }
-    Tensor bits;
-    if (relu && keep)
-        bits = torch::empty({M, blocks_of(N) * 16}, bytes_on(x));
     if (M > 0)
-        gemm(xq, wq, K, bias, relu, y,
-             bits.defined() ? bits.data_ptr<uint8_t>() : nullptr);
-    if (keep) *keep = {xq.q, xq.scale, wt.q, wt.scale, bits};
+        gemm(xq, wq, K, bias, relu, y, relu && keep ? kept + at.bits : nullptr);
     return y;
 }
 
@@ -347,14 +377,15 @@ struct LinearGrads {
 };
 
 // each gradient only where its dtype is given
-LinearGrads linear_bwd(const Tensor& dy, const LinearSaved& s, int64_t K,
+LinearGrads linear_bwd(const Tensor& dy, const Tensor& keep, int64_t K, bool relu,
                        c10::optional<at::ScalarType> dx_type,
                        c10::optional<at::ScalarType> dw_type,
                        c10::optional<at::ScalarType> db_type) {
     check_rows(dy, "dy");
     type_code(dy.scalar_type(), "dy");
     const int64_t M = dy.size(0), N = dy.size(1);
-    TORCH_CHECK(s.xq.size(0) == M, "dy has ", M, " rows and x ", s.xq.size(0));
+    const Kept at(M, N, K, dx_type.has_value(), relu);
+    TORCH_CHECK(keep.size(0) == at.size, "dy does not have the result's rows");
     c10::cuda::CUDAGuard guard(dy.device());
     LinearGrads o;
     if (dx_type) o.dx = torch::empty({M, K}, dy.options().dtype(*dx_type));
@@ -365,29 +396,37 @@ LinearGrads linear_bwd(const Tensor& dy, const LinearSaved& s, int64_t K,
         if (db_type) o.db.zero_();
         return o;
     }
-    Blocks g = quant_rows(
-        dy, s.bits.defined() ? s.bits.data_ptr<uint8_t>() : nullptr,
-        db_type ? &o.db : nullptr);
-    if (dx_type) {
-        Blocks wt{s.wtq, s.wts, K, 128};
-        gemm(g, wt, N, c10::nullopt, false, o.dx, nullptr);
-    }
-    if (dw_type) {
-        // shares of the rows for each tile of 256 x 128: as many as two
-        // workgroups a CU make one round of, with at least 256 rows each
-        const int64_t tiles = (blocks_of(N) + 1) / 2 * blocks_of(K);
-        const int shares = (int)std::max<int64_t>(
-            1, std::min<int64_t>(std::min<int64_t>(512 / tiles, M / 256), 64));
-        Tensor part;
-        if (shares > 1) part = torch::empty({shares, N, K}, floats_on(dy));
+    // shares of the rows for each tile of 256 x 128 of dw: as many as two
+    // workgroups a CU make one round of, with at least 256 rows each
+    const int64_t tiles = (blocks_of(N) + 1) / 2 * blocks_of(K);
+    const int shares = (int)std::max<int64_t>(
+        1, std::min<int64_t>(std::min<int64_t>(512 / tiles, M / 256), 64));
+    const int groups = db_type ? sum_groups(M, N) : quant_groups(M, N, 65535);
+    Carve c;
+    const auto g_at = c.matrix(M, N, 1);
+    const int64_t sum_at = c.take(db_type ? groups * N * 4 : 0);
+    const int64_t part_at = c.take(dw_type && shares > 1 ? shares * N * K * 4 : 0);
+    Tensor work = torch::empty({c.size}, bytes_on(dy));
+    auto* const base = work.data_ptr<uint8_t>();
+    auto* const kept = keep.data_ptr<uint8_t>();
+    const Mat g = mat_at(base, g_at, M, 1), x = mat_at(kept, at.x, M, 1);
+    float* const sums = db_type ? (float*)(base + sum_at) : nullptr;
+    quant_rows(dy, relu ? kept + at.bits : nullptr, g, sums, groups);
+    if (db_type)
+        launched(riqn_column_sum(sums, o.db.data_ptr(),
+                                 type_code(*db_type, "bias"), groups, (int)N,
+                                 stream_of(dy)),
+                 "column sum");
+    if (dx_type)
+        gemm(g, mat_at(kept, at.wt, K, 128), N, c10::nullopt, false, o.dx,
+             nullptr);
+    if (dw_type)
         launched(riqn_fp8_wgrad(
-                     g.q.data_ptr<uint8_t>(), g.scale.data_ptr<uint8_t>(),
-                     s.xq.data_ptr<uint8_t>(), s.xs.data_ptr<uint8_t>(),
-                     o.dw.data_ptr(), type_code(*dw_type, "weight"),
-                     shares > 1 ? part.data_ptr<float>() : nullptr, shares,
+                     g.q, g.scale, x.q, x.scale, o.dw.data_ptr(),
+                     type_code(*dw_type, "weight"),
+                     shares > 1 ? (float*)(base + part_at) : nullptr, shares,
                      (int)M, (int)N, (int)K, stream_of(dy)),
                  "linear_fp8_blocks backward");
-    }
     return o;
 }
 
@@ -398,15 +437,16 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor x,
                           Tensor w, OptTensor bias, bool relu, bool ndx,
                           bool ndw, bool ndb) {
-        const Tensor x2 = as_rows(x);
-        LinearSaved s;
-        Tensor y = linear_fwd(x2, as_rows(w), bias, relu, ndx, &s);
-        ctx->save_for_backward({s.xq, s.xs, s.wtq, s.wts, s.bits});
-        auto& d = ctx->saved_data;
-        d["shape"] = x.sizes().vec();
-        d["dx"] = ndx ? (int64_t)x.scalar_type() : -1;
-        d["dw"] = ndw ? (int64_t)w.scalar_type() : -1;
-        d["db"] = ndb ? (int64_t)bias->scalar_type() : -1;
+        Tensor keep;
+        Tensor y = linear_fwd(as_rows(x), as_rows(w), bias, relu, ndx, &keep);
+        ctx->save_for_backward({keep});
+        // the relu, then the types of the gradients, then x's shape
+        std::vector<int64_t> d = {
+            relu, ndx ? (int64_t)x.scalar_type() : -1,
+            ndw ? (int64_t)w.scalar_type() : -1,
+            ndb ? (int64_t)bias->scalar_type() : -1};
+        d.insert(d.end(), x.sizes().begin(), x.sizes().end());
+        ctx->saved_data["all"] = std::move(d);
         return shaped(y, with_last(x, w.size(0)));
     }
     static torch::autograd::variable_list backward(
@@ -414,17 +454,15 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
         torch::autograd::variable_list dy) {
         check_capture(dy[0]);
         const auto v = ctx->get_saved_variables();
-        auto& d = ctx->saved_data;
-        const auto shape = d["shape"].toIntVector();
-        auto type = [&](const char* n) -> c10::optional<at::ScalarType> {
-            const int64_t t = d[n].toInt();
-            if (t < 0) return c10::nullopt;
-            return (at::ScalarType)t;
+        const auto d = ctx->saved_data["all"].toIntVector();
+        auto type = [&](int i) -> c10::optional<at::ScalarType> {
+            if (d[i] < 0) return c10::nullopt;
+            return (at::ScalarType)d[i];
         };
-        LinearGrads g = linear_bwd(as_rows(dy[0]), {v[0], v[1], v[2], v[3], v[4]},
-                                   shape.back(), type("dx"), type("dw"),
-                                   type("db"));
-        if (g.dx.defined()) g.dx = shaped(g.dx, shape);
+        LinearGrads g = linear_bwd(as_rows(dy[0]), v[0], d.back(), d[0], type(1),
+                                   type(2), type(3));
+        if (g.dx.defined())
+            g.dx = shaped(g.dx, c10::IntArrayRef(d).slice(4));
         return once({g.dx, g.dw, g.db, Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
@@ -468,8 +506,7 @@ Tensor linear_fp8_serve(Tensor x0, Tensor wq, Tensor ws, int64_t block_rows,
                      stream_of(x)),
                  "linear_fp8_blocks");
     else if (y.numel() > 0)
-        gemm(quant_rows(x, nullptr, nullptr), w, x.size(1), bias, relu, y,
-             nullptr);
+        gemm(quant_rows(x).mat(), w.mat(), x.size(1), bias, relu, y, nullptr);
     return shaped(y, with_last(x0, w.rows));
 }
 
@@ -488,26 +525,27 @@ int norm_weights(const Tensor& x, const OptTensor& w, const OptTensor& b) {
     return wt < 0 ? xt : wt;
 }
 
-// mean and rstd: null where no backward pass will ask for them
+// stats gets each row's mean, then each row's rstd; null where no backward pass
+// will ask for them
 Tensor norm_fwd(const Tensor& x, const OptTensor& w, const OptTensor& b,
-                double eps, Tensor* mean, Tensor* rstd) {
+                double eps, Tensor* stats) {
     check_rows(x, "x");
     TORCH_CHECK(x.size(1) >= 1, "x must have at least one column");
     TORCH_CHECK(eps >= 0.0, "eps must not be negative");
     const int wt = norm_weights(x, w, b);
     c10::cuda::CUDAGuard guard(x.device());
     Tensor y = torch::empty({x.size(0), x.size(1)}, x.options());
-    if (mean) {
-        *mean = torch::empty({x.size(0)}, floats_on(x));
-        *rstd = torch::empty({x.size(0)}, floats_on(x));
+    float* mean = nullptr;
+    if (stats) {
+        *stats = torch::empty({2 * x.size(0)}, floats_on(x));
+        mean = stats->data_ptr<float>();
     }
     if (x.size(0) > 0)
         launched(riqn_norm_fwd(
                      x.data_ptr(), type_code(x.scalar_type(), "x"), x.stride(0),
                      w ? w->data_ptr() : nullptr, b ? b->data_ptr() : nullptr,
-                     wt, y.data_ptr(), mean ? mean->data_ptr<float>() : nullptr,
-                     rstd ? rstd->data_ptr<float>() : nullptr, (int)x.size(0),
-                     (int)x.size(1), (float)eps, stream_of(x)),
+                     wt, y.data_ptr(), mean, mean ? mean + x.size(0) : nullptr,
+                     (int)x.size(0), (int)x.size(1), (float)eps, stream_of(x)),
                  "layer_norm");
     return y;
 }
@@ -518,13 +556,14 @@ class NormFn : public torch::autograd::Function<NormFn> {
                           OptTensor w, OptTensor b, double eps, bool ndx,
                           bool ndw, bool ndb) {
         const Tensor x2 = as_rows(x);
-        Tensor mean, rstd;
-        Tensor y = norm_fwd(x2, w, b, eps, &mean, &rstd);
-        ctx->save_for_backward({x2, w ? *w : Tensor(), mean, rstd});
-        auto& d = ctx->saved_data;
-        d["shape"] = x.sizes().vec();
-        d["wtype"] = (int64_t)(w ? *w : b ? *b : x).scalar_type();
-        d["need"] = (int64_t)(ndx | ndw << 1 | ndb << 2);
+        Tensor stats;
+        Tensor y = norm_fwd(x2, w, b, eps, &stats);
+        ctx->save_for_backward({x2, w ? *w : Tensor(), stats});
+        // which gradients, their type, then x's shape
+        std::vector<int64_t> d = {ndx | ndw << 1 | ndb << 2,
+                                  (int64_t)(w ? *w : b ? *b : x).scalar_type()};
+        d.insert(d.end(), x.sizes().begin(), x.sizes().end());
+        ctx->saved_data["all"] = std::move(d);
         return shaped(y, x.sizes());
     }
     static torch::autograd::variable_list backward(
@@ -532,10 +571,11 @@ class NormFn : public torch::autograd::Function<NormFn> {
         torch::autograd::variable_list grad) {
         check_capture(grad[0]);
         const auto v = ctx->get_saved_variables();
-        const Tensor &x = v[0], &w = v[1], &mean = v[2], &rstd = v[3];
-        auto& d = ctx->saved_data;
-        const int64_t need = d["need"].toInt();
-        const auto w_type = (at::ScalarType)d["wtype"].toInt();
+        const Tensor &x = v[0], &w = v[1];
+        const float* const mean = v[2].data_ptr<float>();
+        const auto d = ctx->saved_data["all"].toIntVector();
+        const int64_t need = d[0];
+        const auto w_type = (at::ScalarType)d[1];
         const Tensor dy = as_rows(grad[0]);
         TORCH_CHECK(dy.sizes() == x.sizes() && dy.device() == x.device() &&
                         dy.scalar_type() == x.scalar_type(),
@@ -557,8 +597,7 @@ class NormFn : public torch::autograd::Function<NormFn> {
                          dy.data_ptr(), x.data_ptr(),
                          type_code(x.scalar_type(), "x"), dy.stride(0),
                          x.stride(0), w.defined() ? w.data_ptr() : nullptr,
-                         type_code(w_type, "weight"), mean.data_ptr<float>(),
-                         rstd.data_ptr<float>(),
+                         type_code(w_type, "weight"), mean, mean + R,
                          need & 1 ? dx.data_ptr() : nullptr,
                          need & 2 ? dw.data_ptr() : nullptr,
                          need & 4 ? db.data_ptr() : nullptr,
@@ -566,7 +605,7 @@ class NormFn : public torch::autograd::Function<NormFn> {
                          (int)R, (int)C, stream_of(x)),
                      "layer_norm backward");
         }
-        if (need & 1) dx = shaped(dx, d["shape"].toIntVector());
+        if (need & 1) dx = shaped(dx, c10::IntArrayRef(d).slice(2));
         return once({dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
@@ -574,8 +613,7 @@ class NormFn : public torch::autograd::Function<NormFn> {
 Tensor layer_norm(Tensor x, OptTensor w, OptTensor b, double eps) {
     if (!at::GradMode::is_enabled() ||
         !(wants_grad(x) || wants_grad(w) || wants_grad(b)))
-        return shaped(norm_fwd(as_rows(x), w, b, eps, nullptr, nullptr),
-                      x.sizes());
+        return shaped(norm_fwd(as_rows(x), w, b, eps, nullptr), x.sizes());
     return NormFn::apply(x, w, b, eps, wants_grad(x), wants_grad(w),
                          wants_grad(b));
 }
