@@ -613,6 +613,69 @@ DEV __amdgpu_buffer_rsrc_t buffer_of(const uint8_t* p, int64_t bytes) {
         (void*)p, 0, (int)min(bytes, (int64_t)0xffffffffu), 0x00027000);
 }
 
+// B's row at place r of a tile, see above
+DEV int place_b(int r) {
+    return (r & ~31) + ((r & 15) >> 2) * 8 + ((r >> 4) & 1) * 4 + (r & 3);
+}
+
+// The results of a wave: columns n ... n + 7 of rows m0 + 16 i + lane % 16, for
+// each 32 columns.  A row's stores follow each other, so that whole lines are
+// written.
+template <int MI, int NJ, typename T>
+DEV void store_tile(const Gemm& g, const f32x4 (&acc)[MI][NJ], int m0, int n0,
+                    int lane) {
+    const int l15 = lane & 15, l4 = lane >> 4;
+    const bool even = (g.N & 7) == 0;  // all 8 there, and aligned
+    auto finish = [&](auto plain, const float (&bias)[NJ / 2][8]) {
+        #pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int m = m0 + i * 16 + l15;
+            #pragma unroll
+            for (int c = 0; c < NJ / 2; ++c) {
+                const int n = n0 + c * 32 + l4 * 8;
+                unsigned bits = 0;
+                struct alignas(16) Pack { T t[8]; } p;
+                #pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float z = acc[i][c * 2 + (e >> 2)][e & 3];
+                    if (!decltype(plain)::value) {
+                        z += bias[c][e];
+                        const bool on = passes(z);
+                        bits |= (unsigned)(on && n + e < g.N) << e;
+                        if (g.relu && !on) z = 0.0f;
+                    }
+                    p.t[e] = from_f<T>(z);
+                }
+                if (m >= g.M || n >= g.N) continue;
+                if (!decltype(plain)::value && g.mask)
+                    g.mask[(int64_t)m * (((g.N + 127) >> 7) * 16) + (n >> 3)] =
+                        (uint8_t)bits;
+                T* out = (T*)g.c + (int64_t)m * g.N + n;
+                if (even) {
+                    *(Pack*)out = p;
+                } else {
+                    #pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (n + e < g.N) out[e] = p.t[e];
+                }
+            }
+        }
+    };
+    // without any of them the results go out as they are: the rest is 10
+    // instructions a value, as long as 4 steps of products
+    float bias[NJ / 2][8];
+    if (g.bias || g.relu || g.mask) {
+        #pragma unroll
+        for (int c = 0; c < NJ / 2; ++c)
+            #pragma unroll
+            for (int e = 0; e < 8; ++e)
+                bias[c][e] = bias_at(g, min(n0 + c * 32 + l4 * 8 + e, g.N - 1));
+        finish(std::false_type{}, bias);
+    } else {
+        finish(std::true_type{}, bias);
+    }
+}
+
 template <int WM, int WN, int MI, int NJ, bool EXACT, typename T>
 __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host needs its launch alone
@@ -644,10 +707,6 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
     constexpr int LA = TM / 8 / WAVES, LB = TN / 8 / WAVES;
     __amdgpu_buffer_rsrc_t buf_a, buf_b, buf_s;
     uint32_t off[LA + LB], off_s;
-    // B's row at place r of a tile, see above
-    auto place = [](int r) {
-        return (r & ~31) + ((r & 15) >> 2) * 8 + ((r >> 4) & 1) * 4 + (r & 3);
-    };
     auto enter = [&](int tile) {
         const int m0 = (tile / nt) * TM, n0 = (tile % nt) * TN;
         buf_a = buffer_of(g.a + m0 * ld, (g.M - m0) * ld);
@@ -657,7 +716,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
             const int inst = (i < LA ? i : i - LA) * WAVES + wave;
             const int r = inst * 8 + (lane >> 3);
             const int from = i < LA ? min(r, g.M - 1 - m0)
-                                    : min(place(r), g.N - 1 - n0);
+                                    : min(place_b(r), g.N - 1 - n0);
             off[i] = (uint32_t)from * (uint32_t)ld +
                      ((lane & 7) ^ ((r >> 1) & 7)) * 16;
         }
@@ -672,7 +731,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
             const int r0 = n0 >> g.bsh;
             buf_s = buffer_of(g.bs + (int64_t)r0 * g.S,
                               (((g.N - 1) >> g.bsh) + 1 - r0) * (int64_t)g.S);
-            off_s = (((n0 + min(place(r - TM), g.N - 1 - n0)) >> g.bsh) - r0) * g.S;
+            off_s = (((n0 + min(place_b(r - TM), g.N - 1 - n0)) >> g.bsh) - r0) * g.S;
         }
     };
     int sbuf = 1;  // which scales are in use
@@ -805,57 +864,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(Gemm g) {
         // The next tile's first step is waited for here: behind the stores it
         // would be waited for with them, as the counter knows one order only.
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        // columns n ... n + 7 of rows m0 + 16 i + l15, for each 32 columns; a
-        // row's stores follow each other, so that whole lines are written
-        const bool even = (g.N & 7) == 0;  // all 8 there, and aligned
-        auto finish = [&](auto plain, const float (&bias)[NJ / 2][8]) {
-            #pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                const int m = m0 + i * 16 + l15;
-                #pragma unroll
-                for (int c = 0; c < NJ / 2; ++c) {
-                    const int n = n0 + c * 32 + l4 * 8;
-                    unsigned bits = 0;
-                    struct alignas(16) Pack { T t[8]; } p;
-                    #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float z = acc[i][c * 2 + (e >> 2)][e & 3];
-                        if (!decltype(plain)::value) {
-                            z += bias[c][e];
-                            const bool on = passes(z);
-                            bits |= (unsigned)(on && n + e < g.N) << e;
-                            if (g.relu && !on) z = 0.0f;
-                        }
-                        p.t[e] = from_f<T>(z);
-                    }
-                    if (m >= g.M || n >= g.N) continue;
-                    if (!decltype(plain)::value && g.mask)
-                        g.mask[(int64_t)m * (((g.N + 127) >> 7) * 16) + (n >> 3)] =
-                            (uint8_t)bits;
-                    T* out = (T*)g.c + (int64_t)m * g.N + n;
-                    if (even) {
-                        *(Pack*)out = p;
-                    } else {
-                        #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (n + e < g.N) out[e] = p.t[e];
-                    }
-                }
-            }
-        };
-        // without any of them the results go out as they are: the rest is 10
-        // instructions a value, as long as 4 steps of products
-        float bias[NJ / 2][8];
-        if (g.bias || g.relu || g.mask) {
-            #pragma unroll
-            for (int c = 0; c < NJ / 2; ++c)
-                #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    bias[c][e] = bias_at(g, min(n0 + c * 32 + l4 * 8 + e, g.N - 1));
-            finish(std::false_type{}, bias);
-        } else {
-            finish(std::true_type{}, bias);
-        }
+        store_tile<MI, NJ, T>(g, acc, m0, n0, lane);
     }
     // no load may come in after the workgroup has given its LDS back
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -877,6 +886,163 @@ void launch_tiles(const Gemm& g, hipStream_t st) {
     else
         hipLaunchKernelGGL((gemm_tile_kernel<WM, WN, MI, NJ, sizeof(T) == 4, T>),
                            grid, dim3(64 * WM * WN), bytes, st, g);
+}
+
+// The same for fewer results, where a workgroup or two fall to a CU and a step
+// takes as long as the way from one barrier to the next: loads, LDS reads and
+// products one behind the other.  One tile of 64 x 64 a workgroup; two groups
+// of 4 waves take every other step, so that there are half as many barriers and
+// one group's reads go on under the other's products.  Their sums are added at
+// the end, through LDS.  [1024, 1024, 3136]: 9.3 us in bf16, 13.7 in fp32; with
+// one group 11.9 and 16.0, with four 9.7 and 13.4.
+template <bool EXACT, typename T>
+__global__ __launch_bounds__(512) void gemm_shared_kernel(Gemm g) {
+#ifdef __HIP_DEVICE_COMPILE__
+    constexpr int TM = 64, TN = 64, MI = 2, NJ = 2, WAVES = 4, LOADS = 4;
+    // a step's rows, then the dwords of scales of them
+    constexpr int BUF = (TM + TN) * (128 + 4);
+    extern __shared__ __align__(16) uint8_t lds[];  // [2 buffers][2 groups][BUF]
+    const int lane = threadIdx.x & 63;
+    const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = all / WAVES, wave = all % WAVES;
+    const int l15 = lane & 15, l4 = lane >> 4;
+    const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
+    const int nt = (g.N + TN - 1) / TN;
+    const int64_t ld = (int64_t)g.nb * 128;
+    // each XCD takes one run of tiles, as above
+    const int xcd = blockIdx.x & 7, q = gridDim.x >> 3, rem = gridDim.x & 7;
+    const int tile = xcd * q + min(xcd, rem) + (blockIdx.x >> 3);
+    const int m0 = (tile / nt) * TM, n0 = (tile % nt) * TN;
+    const auto buf_a = buffer_of(g.a + m0 * ld, (g.M - m0) * ld);
+    const auto buf_b = buffer_of(g.b + n0 * ld, (g.N - n0) * ld);
+    uint32_t off[LOADS];  // A, A, B, B
+    #pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int r = ((i & 1) * WAVES + wave) * 8 + (lane >> 3);
+        const int from = i < 2 ? min(r, g.M - 1 - m0)
+                               : min(place_b(r), g.N - 1 - n0);
+        off[i] = (uint32_t)from * (uint32_t)ld +
+                 ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+    }
+    // scales: wave 0 takes those of A's rows, wave 1 those of B's
+    const int r0 = wave ? n0 >> g.bsh : m0 >> g.ash;
+    const int rows = wave ? ((g.N - 1) >> g.bsh) + 1 : ((g.M - 1) >> g.ash) + 1;
+    const auto buf_s = buffer_of((wave ? g.bs : g.as) + (int64_t)r0 * g.S,
+                                 (rows - r0) * (int64_t)g.S);
+    const uint32_t off_s =
+        (wave ? ((n0 + min(place_b(lane), g.N - 1 - n0)) >> g.bsh) - r0
+              : (min(m0 + lane, g.M - 1) >> g.ash) - r0) * g.S;
+    typedef __attribute__((address_space(3))) void* lds_t;
+    // a group's step of a round; behind the last one the last, for nothing
+    auto stage = [&](int round) {
+        const int kb = min(round * 2 + group, g.nb - 1);
+        uint8_t* const to = lds + ((round & 1) * 2 + group) * BUF;
+        if (wave < 2)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                buf_s, (lds_t)(to + (TM + TN) * 128 + wave * 256), 4, off_s,
+                kb & ~3, 0, 0);
+        #pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                i < 2 ? buf_a : buf_b,
+                (lds_t)(to + (i < 2 ? 0 : TM * 128) +
+                        ((i & 1) * WAVES + wave) * 1024),
+                16, off[i], kb * 128, 0, 0);
+    };
+    f32x4 acc[MI][NJ];
+    #pragma unroll
+    for (int i = 0; i < MI; ++i)
+        #pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    stage(0);
+    for (int round = 0; round * 2 < g.nb; ++round) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        stage(round + 1);  // into the buffer that all are past reading
+        const int kb = round * 2 + group;
+        if (kb >= g.nb) continue;
+        const uint8_t* A = lds + ((round & 1) * 2 + group) * BUF;
+        const uint8_t* B = A + TM * 128;
+        const uint32_t* sc = (const uint32_t*)(A + (TM + TN) * 128);
+        auto piece = [&](const uint8_t* base, int row, int p) {
+            return *(const i32x4*)(base + row * 128 +
+                                   ((p ^ ((row >> 1) & 7)) * 16));
+        };
+        const int shift = (kb & 3) * 8;
+        int ea[MI], eb[NJ];
+        i32x4 fa[MI][2], fb[NJ][2];
+        #pragma unroll
+        for (int i = 0; i < MI; ++i)
+            ea[i] = (sc[wm + i * 16 + l15] >> shift) & 255;
+        #pragma unroll
+        for (int j = 0; j < NJ; ++j)
+            eb[j] = (sc[TM + wn + j * 16 + l15] >> shift) & 255;
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            #pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                fb[j][h] = piece(B, wn + j * 16 + l15, h * 4 + l4);
+            #pragma unroll
+            for (int i = 0; i < MI; ++i)
+                fa[i][h] = piece(A, wm + i * 16 + l15, h * 4 + l4);
+        }
+        if (!EXACT) {
+            #pragma unroll
+            for (int i = 0; i < MI; ++i)
+                #pragma unroll
+                for (int j = 0; j < NJ; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        two(fb[j][0], fb[j][1]), two(fa[i][0], fa[i][1]),
+                        acc[i][j], 0, 0, 0, eb[j], 0, ea[i]);
+        } else {
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                #pragma unroll
+                for (int u = 0; u < 4; u += 2) {
+                    bf16x8 xb[NJ];
+                    #pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+                        xb[j] = expand8(fb[j][h][u], fb[j][h][u + 1], eb[j]);
+                    #pragma unroll
+                    for (int i = 0; i < MI; ++i) {
+                        const bf16x8 xa =
+                            expand8(fa[i][h][u], fa[i][h][u + 1], ea[i]);
+                        #pragma unroll
+                        for (int j = 0; j < NJ; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                xb[j], xa, acc[i][j], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+    // no load may come in behind this, over the sums or after the workgroup
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    f32x4* const part = (f32x4*)lds + wave * (MI * NJ * 64) + lane;
+    __syncthreads();
+    if (group == 1) {
+        #pragma unroll
+        for (int i = 0; i < MI * NJ; ++i) part[i * 64] = acc[i / NJ][i % NJ];
+    }
+    __syncthreads();
+    if (group == 1) return;
+    #pragma unroll
+    for (int i = 0; i < MI * NJ; ++i) acc[i / NJ][i % NJ] += part[i * 64];
+    store_tile<MI, NJ, T>(g, acc, m0 + wm, n0 + wn, lane);
+#endif
+}
+
+template <typename T>
+void launch_shared(const Gemm& g, hipStream_t st) {
+    constexpr int bytes = 2 * 2 * (64 + 64) * (128 + 4);
+    const dim3 grid(((g.M + 63) / 64) * ((g.N + 63) / 64));
+    if (sizeof(T) == 4 || g.mask)
+        hipLaunchKernelGGL((gemm_shared_kernel<true, T>), grid, dim3(512), bytes,
+                           st, g);
+    else
+        hipLaunchKernelGGL((gemm_shared_kernel<sizeof(T) == 4, T>), grid,
+                           dim3(512), bytes, st, g);
 }
 
 // ---------------------------------------------------------------------------
@@ -1215,21 +1381,28 @@ int riqn_fp8_gemm(const uint8_t* a, const uint8_t* as, int a_block_rows,
         return (int64_t)((M + t - 1) / t) * ((N + t - 1) / t);
     };
     // The largest tile of which there are enough for the 256 CUs: it moves the
-    // fewest bytes.  Measured in us, tiles of 32 (direct) / 64 / 128 / 256, in
-    // bf16, [M, 1024, 3136]: M = 256: 9 / 12 / 19 / 43, 512: 16 / 12 / 19 / 43,
-    // 4096: 102 / 25 / 25 / 44, 8192: - / 47 / 35 / 48, 16384: - / 91 / 61 /
-    // 54; [M, 3136, 1024]: M = 64: 5 / 6 / 9 / 15, 256: 11 / 6 / 10 / 25,
-    // 1024: 30 / 13 / 12 / 25, 4096: 97 / 33 / 30 / 28.
+    // fewest bytes.  Tiles of 64 that all fit at once, two on a CU, share their
+    // steps out over two groups of waves.  Measured in us, bf16 / fp32 results,
+    // tiles of 32 (direct) | 64 shared | 64 | 128 | 256; [M, 1024, 3136]:
+    //   M =  256    9 /  9 |  9 / 13 | 12 / 15 | 19 / 29 | 43 / 74
+    //       1024   30 /    |  9 / 14 | 12 / 16 | 20 / 30 | 44 / 75
+    //       2048           | 14 / 21 | 18 / 22 | 23 / 31 | 44 / 76
+    //       2900           | 24 / 30 | 20 / 28 | 25 / 32 | 45 / 77
+    //       4096           | 27 / 38 | 23 / 35 | 25 / 33 | 45 / 78
+    //       8192           | 54 / 75 | 47 /    | 32 / 53 | 48 / 80
+    //      16384           |         | 91 /    | 61 /    | 52 / 89
+    // and [30000, 64, 512]:   6 /  8 |  6 /  8 |  7 / 10 | 11 / 17
     RIQN_TYPE(c_type, T, {
         if (M <= 16) {
             hipLaunchKernelGGL((gemm_direct_kernel<1, 1, T>),
                                dim3((N + 15) / 16), dim3(512), 0, st, g);
         } else if (tiles(256) >= 192) {
             launch_tiles<2, 4, 8, 4, T>(g, st);
-        } else if (tiles(128) >= 192) {
-            launch_tiles<2, 2, 4, 4, T>(g, st);
+        } else if (tiles(64) > 512) {
+            if (tiles(128) >= 192) launch_tiles<2, 2, 4, 4, T>(g, st);
+            else launch_tiles<2, 2, 2, 2, T>(g, st);
         } else if (tiles(32) > 256) {
-            launch_tiles<2, 2, 2, 2, T>(g, st);
+            launch_shared<T>(g, st);
         } else {
             hipLaunchKernelGGL((gemm_direct_kernel<2, 2, T>),
                                dim3((uint32_t)tiles(32)), dim3(512), 0, st, g);
