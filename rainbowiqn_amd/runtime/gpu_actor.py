@@ -67,13 +67,16 @@ class GpuActorLoop:
         self.chunk_meta = torch.zeros(c, 3, device=d)
         self.use_graph = use_graph
         self.graph: Optional[torch.cuda.CUDAGraph] = None
+        # its own, as graphs of one capture stream share the math libraries'
+        # workspace, and this one replays beside the learner's
+        self.capture_stream = torch.cuda.Stream(d)
         self.total_steps = 0
         self._newest = 0  # ring slot of the most recent frame (round-invariant)
         # hand-written fused forward (4 kernels/step) on the bf16 path
         self.fused = None
         if (self.dtype == torch.bfloat16
                 and net.fc_h_v.weight_mu.dtype == torch.bfloat16
-                and getattr(cfg, "fused_model", True)):
+                and cfg.fused_model):
             from .fused_forward import FusedForward
 
             self.fused = FusedForward.for_net(
@@ -130,7 +133,7 @@ class GpuActorLoop:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        with torch.cuda.graph(g, stream=self.capture_stream):
             self._round_body()
         self.graph = g
 

@@ -104,13 +104,17 @@ class GpuLearner:
         self.loss_static = torch.zeros(1, device=self.device)
         self.use_graph = use_graph
         self.graph: Optional[torch.cuda.CUDAGraph] = None
+        # a stream of its own: the math libraries keep one workspace a stream,
+        # and graphs captured on the same one would share it.  This one replays
+        # beside the actors'.
+        self.capture_stream = torch.cuda.Stream(self.device)
         self.steps_per_replay = 1
         self.grad_steps = 0
         # fused no-grad forwards (double-Q select + target quantiles): 4
         # hand-written kernels each instead of the eager module stack
         self.fused_online = self.fused_target = None
         self.manual_bwd = False
-        if self.bf16 and getattr(cfg, "fused_model", True):
+        if self.bf16 and cfg.fused_model:
             from .fused_forward import FusedForward
 
             fp8 = getattr(cfg, "fp8_heads", False)
@@ -352,7 +356,7 @@ class GpuLearner:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        with torch.cuda.graph(g, stream=self.capture_stream):
             for _ in range(steps_per_replay):
                 self._step_body()
         self.graph = g

@@ -186,3 +186,20 @@ def test_learner_and_actor(flags, dtype):
     for k, p in runner.glearner.online.named_parameters():
         if k.startswith(("feature_norm", "fc_h")):
             assert p.grad.any(), k
+
+
+@gpu
+def test_graphs_that_replay_side_by_side_share_no_stream():
+    """The math libraries' workspace is a stream's; these graphs hold library
+    products and replay at the same time."""
+    from rainbowiqn_amd.parallel.apex import ApexRunner
+    from rainbowiqn_amd.parallel.comm import Communicator
+
+    cfg = Config(device="cuda", dtype="bf16", learn_start=256, memory_capacity=8192,
+                 learn_per_round=2, cu_split=0, **BOTH)
+    runner = ApexRunner(cfg, Communicator(backend="auto"), n_envs=32, chunk_steps=8)
+    used = [runner.glearner] + list(runner.gactors)
+    streams = {g.capture_stream.cuda_stream for g in used}
+    streams.add(torch.cuda.graph.default_capture_stream.cuda_stream
+                if torch.cuda.graph.default_capture_stream else -1)
+    assert len(streams) == len(used) + 1
