@@ -15,6 +15,10 @@
 
 namespace {
 
+// A memset would become a node of a captured graph that does not replay
+// reliably.
+__global__ void clear_loss_kernel(float* out_loss) { *out_loss = 0.0f; }
+
 __global__ void quantile_huber_kernel(
     const float* __restrict__ theta, const float* __restrict__ target_q,
     const float* __restrict__ taus, const float* __restrict__ returns,
@@ -71,7 +75,7 @@ extern "C" void riqn_quantile_huber(
     float gamma_n, float kappa, int B, int N, int Np, float* out_loss,
     float* out_per_sample, float* out_grad_theta, void* stream) {
     hipStream_t s = (hipStream_t)stream;
-    hipMemsetAsync(out_loss, 0, sizeof(float), s);
+    hipLaunchKernelGGL(clear_loss_kernel, dim3(1), dim3(1), 0, s, out_loss);
     int bt = ((max(N, Np) + 63) / 64) * 64;
     hipLaunchKernelGGL(quantile_huber_kernel, dim3(B), dim3(bt), 0, s, theta,
                        target_q, taus, returns, nonterm, weights, gamma_n,

@@ -203,3 +203,33 @@ def test_graphs_that_replay_side_by_side_share_no_stream():
     streams.add(torch.cuda.graph.default_capture_stream.cuda_stream
                 if torch.cuda.graph.default_capture_stream else -1)
     assert len(streams) == len(used) + 1
+
+
+@gpu
+def test_captured_loss_replays():
+    from rainbowiqn_amd.ops.functional import quantile_huber_loss_fused
+
+    def draw(seed):
+        g = torch.Generator().manual_seed(seed)
+        return [t.cuda() for t in (torch.randn(32, 8, generator=g),
+                                   torch.randn(32, 8, generator=g),
+                                   torch.rand(32, 8, generator=g),
+                                   torch.randn(32, generator=g),
+                                   torch.ones(32), torch.rand(32, generator=g))]
+
+    args = draw(0)
+    one = lambda: quantile_huber_loss_fused(*args, 0.99, 3)  # noqa: E731
+    one()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, per = one()
+    for i in range(1, 6):
+        for t, new in zip(args, draw(i)):
+            t.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, want_per = one()
+        assert torch.equal(per, want_per)
+        # added up by atomics: 32 terms of one sign in any order
+        assert abs(float(loss - want)) <= 64 * 2.0 ** -24 * float(want)
