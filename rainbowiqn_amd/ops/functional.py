@@ -128,8 +128,8 @@ def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> Fp8Blocks:
     scaling is exact and the values lose only digits past the fourth
     significant bit (a relative error of 2^-4 at most down to 2^-13 of the
     block's largest value).  Values that are not finite become NaN."""
-    x = x.detach()
     if not x.is_cuda:
+        x = x.detach()
         _check_matrix(x, "x")
         if block_rows not in (1, 128):
             raise RuntimeError("block_rows must be 1 or 128")
@@ -156,7 +156,11 @@ def matmul_fp8_blocks(a: Fp8Blocks, b: Fp8Blocks,
                       bias: Optional[torch.Tensor] = None, relu: bool = False,
                       out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """a b^T (+ bias, relu): a [M, K], b [N, K], bias [N] -> [M, N].  Sums in
-    fp32, rounded once to `out_dtype`."""
+    fp32, rounded once to `out_dtype`.
+
+    float32: exact products (of values under 2^-126 what bfloat16 keeps of
+    them).  bfloat16, float16: products of more than a few rows may be cut at
+    2^-13 of the largest of 8 neighbours."""
     if a.cols != b.cols:
         raise RuntimeError(f"a has {a.cols} columns and b {b.cols}")
     if not a.q.is_cuda:

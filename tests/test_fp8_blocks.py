@@ -673,3 +673,59 @@ def test_the_same_tensor_twice():
     twin = blocks._replace(q=blocks.q.clone(), scale=blocks.scale.clone())
     assert torch.equal(F.matmul_fp8_blocks(blocks, blocks),
                        F.matmul_fp8_blocks(blocks, twin))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [
+    # tiles of 64 that two groups of waves share: 1 to 5 steps, so that one
+    # group has none or one less
+    (1037, 517, 1), (1037, 517, 129), (1000, 513, 257), (640, 1025, 400),
+    (1037, 517, 600),
+    # tiles of 256: odd in every size, one step, and results of 4 in a row
+    (12001, 1101, 200), (7000, 2005, 100), (9001, 1412, 385), (12550, 1024, 520)])
+def test_product_in_more_tiles(m, n, k, dtype):
+    """The same bounds as above, at sizes that other tiles are chosen for."""
+    x = (0.25 * matrix(m, k, 1)).clamp(-8, 8)
+    w = torch.rand(n, k, generator=torch.Generator().manual_seed(2)) - 0.5
+    bias = matrix(1, n, 3)[0].clamp(-1, 1).to(dtype).cuda()
+    a, b = F.quantize_fp8_blocks(x.cuda()), F.quantize_fp8_blocks(w.cuda(), 128)
+    xh, wh = held(x).cuda(), held(w, 128).cuda()
+    z, size = (xh @ wh.t()).cpu(), (xh.abs() @ wh.abs().t()).cpu()
+    near(F.matmul_fp8_blocks(a, b, out_dtype=dtype), z, tol(k, size, z, dtype))
+    z, size = z + bias.double().cpu(), size + bias.double().cpu().abs()
+    near(F.matmul_fp8_blocks(a, b, bias, True, dtype), z.clamp(min=0),
+         tol(k + 1, size, z, dtype))
+
+
+@gpu
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("m,n,k", [(12501, 1030, 140), (7001, 140, 2061)])
+def test_linear_in_more_tiles(m, n, k, relu):
+    """Tiles of 256 forward, with the relu's bits, and for dx."""
+    x = (0.25 * matrix(m, k, 1)).clamp(-8, 8).bfloat16().cuda().requires_grad_()
+    w = torch.rand(n, k, generator=torch.Generator().manual_seed(2)) - 0.5
+    w = w.bfloat16().cuda().requires_grad_()
+    b = matrix(1, n, 3)[0].clamp(-1, 1).bfloat16().cuda().requires_grad_()
+    dy = (0.1 * matrix(m, n, 4)).clamp(-2, 2).bfloat16().cuda()
+    y = F.linear_fp8_blocks(x, w, b, relu)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    check_linear(x, w, b, dy, y, dx, dw, db, relu)
+
+
+def no_gradient_through(device):
+    x = matrix(5, 200, 1, device=device).requires_grad_()
+    for t in (x, x.t().contiguous().t(), x * 2):
+        b = F.quantize_fp8_blocks(t)
+        assert not b.q.requires_grad and not b.scale.requires_grad
+        assert not F.dequantize_fp8_blocks(b).requires_grad
+        assert not F.matmul_fp8_blocks(b, b).requires_grad
+
+
+def test_no_gradient_through_blocks_cpu():
+    no_gradient_through("cpu")
+
+
+@gpu
+def test_no_gradient_through_blocks_gpu():
+    no_gradient_through("cuda")
