@@ -364,3 +364,20 @@ def test_infinite_weight_stays_in_its_column(cols):
     same = (h * h[:, -1:] > 0)[:, :-1]
     assert torch.equal(dx[:, :-1].isnan(), ~same)
     assert dx[:, :-1][same].isinf().all()
+
+
+@gpu
+@pytest.mark.parametrize("types", [(torch.float32,) * 2, (torch.bfloat16,) * 2,
+                                   (torch.float16, torch.float32)])
+@pytest.mark.parametrize("cols", [1, 7, 8, 9, 15, 503, 505, 511, 513, 1023, 1025,
+                                  2047, 2049, 4089, 4095, 4097])
+def test_odd_columns(cols, types):
+    """Rows whose end and beginning lie anywhere, where two lanes have the last
+    columns."""
+    wide, w, b, wide_dy = inputs(37, cols + 3, *types, "cuda")
+    x = wide.detach()[:, 3:].requires_grad_()
+    w, b = (t.detach()[3:].clone().requires_grad_() for t in (w, b))
+    dy = wide_dy[:, 1:cols + 1]
+    got = step(x, w, b, dy)
+    for name, (want, bound) in plain(x, w, b, 1e-5, dy).items():
+        near(got[name], want, bound)
