@@ -195,12 +195,12 @@ Blocks quant_tiles(const Tensor& x) {
 }
 
 void gemm(const Mat& a, const Mat& b, int64_t K, const OptTensor& bias,
-          bool relu, Tensor& c, uint8_t* mask) {
+          bool relu, Tensor& c, uint8_t* mask, bool exact) {
     launched(riqn_fp8_gemm(
                  a.q, a.scale, (int)a.block_rows, b.q, b.scale,
                  (int)b.block_rows, bias ? bias->data_ptr() : nullptr,
                  bias ? type_code(bias->scalar_type(), "bias") : 0, relu,
-                 c.data_ptr(), type_code(c.scalar_type(), "out"), mask,
+                 c.data_ptr(), type_code(c.scalar_type(), "out"), mask, exact,
                  (int)a.rows, (int)b.rows, (int)K, stream_of(c)),
              "matmul_fp8_blocks");
 }
@@ -233,7 +233,8 @@ Tensor fp8_blocks_dequant(Tensor q, Tensor scale, int64_t cols,
 
 Tensor fp8_blocks_matmul(Tensor aq, Tensor as, int64_t a_block_rows, Tensor bq,
                          Tensor bs, int64_t b_block_rows, int64_t cols,
-                         OptTensor bias, bool relu, at::ScalarType dtype) {
+                         OptTensor bias, bool relu, at::ScalarType dtype,
+                         bool exact) {
     Blocks a = check_blocks(aq, as, cols, a_block_rows, "a");
     Blocks b = check_blocks(bq, bs, cols, b_block_rows, "b");
     TORCH_CHECK(aq.device() == bq.device(), "a and b must be on one GPU");
@@ -245,7 +246,7 @@ Tensor fp8_blocks_matmul(Tensor aq, Tensor as, int64_t a_block_rows, Tensor bq,
     c10::cuda::CUDAGuard guard(aq.device());
     Tensor c = torch::empty({a.rows, b.rows}, aq.options().dtype(dtype));
     if (c.numel() == 0) return c;
-    gemm(a.mat(), b.mat(), cols, bias, relu, c, nullptr);
+    gemm(a.mat(), b.mat(), cols, bias, relu, c, nullptr, exact);
     return c;
 }
 
@@ -325,7 +326,7 @@ struct Kept {
 
 // y = x W^T + bias, relu; `keep` gets what the backward pass reads (Kept)
 Tensor linear_fwd(const Tensor& x, const Tensor& w, const OptTensor& bias,
-                  bool relu, bool need_dx, Tensor* keep) {
+                  bool relu, bool exact, bool need_dx, Tensor* keep) {
     check_rows(x, "x");
     check_rows(w, "weight");
     TORCH_CHECK(w.device() == x.device(), "weight must be on ", x.device());
@@ -368,7 +369,8 @@ Tensor linear_fwd(const Tensor& x, const Tensor& w, const OptTensor& bias,
                  "linear_fp8_blocks");
     }
     if (M > 0)
-        gemm(xq, wq, K, bias, relu, y, relu && keep ? kept + at.bits : nullptr);
+        gemm(xq, wq, K, bias, relu, y, relu && keep ? kept + at.bits : nullptr,
+             exact);
     return y;
 }
 
@@ -378,7 +380,7 @@ struct LinearGrads {
 
 // each gradient only where its dtype is given
 LinearGrads linear_bwd(const Tensor& dy, const Tensor& keep, int64_t K, bool relu,
-                       c10::optional<at::ScalarType> dx_type,
+                       bool exact, c10::optional<at::ScalarType> dx_type,
                        c10::optional<at::ScalarType> dw_type,
                        c10::optional<at::ScalarType> db_type) {
     check_rows(dy, "dy");
@@ -419,7 +421,7 @@ LinearGrads linear_bwd(const Tensor& dy, const Tensor& keep, int64_t K, bool rel
                  "column sum");
     if (dx_type)
         gemm(g, mat_at(kept, at.wt, K, 128), N, c10::nullopt, false, o.dx,
-             nullptr);
+             nullptr, exact);
     if (dw_type)
         launched(riqn_fp8_wgrad(
                      g.q, g.scale, x.q, x.scale, o.dw.data_ptr(),
@@ -435,14 +437,15 @@ LinearGrads linear_bwd(const Tensor& dy, const Tensor& keep, int64_t K, bool rel
 class LinearFn : public torch::autograd::Function<LinearFn> {
   public:
     static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor x,
-                          Tensor w, OptTensor bias, bool relu, bool ndx,
-                          bool ndw, bool ndb) {
+                          Tensor w, OptTensor bias, bool relu, bool exact,
+                          bool ndx, bool ndw, bool ndb) {
         Tensor keep;
-        Tensor y = linear_fwd(as_rows(x), as_rows(w), bias, relu, ndx, &keep);
+        Tensor y =
+            linear_fwd(as_rows(x), as_rows(w), bias, relu, exact, ndx, &keep);
         ctx->save_for_backward({keep});
-        // the relu, then the types of the gradients, then x's shape
+        // the relu, exactness, the types of the gradients, then x's shape
         std::vector<int64_t> d = {
-            relu, ndx ? (int64_t)x.scalar_type() : -1,
+            relu, exact, ndx ? (int64_t)x.scalar_type() : -1,
             ndw ? (int64_t)w.scalar_type() : -1,
             ndb ? (int64_t)bias->scalar_type() : -1};
         d.insert(d.end(), x.sizes().begin(), x.sizes().end());
@@ -459,28 +462,29 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
             if (d[i] < 0) return c10::nullopt;
             return (at::ScalarType)d[i];
         };
-        LinearGrads g = linear_bwd(as_rows(dy[0]), v[0], d.back(), d[0], type(1),
-                                   type(2), type(3));
+        LinearGrads g = linear_bwd(as_rows(dy[0]), v[0], d.back(), d[0], d[1],
+                                   type(2), type(3), type(4));
         if (g.dx.defined())
-            g.dx = shaped(g.dx, c10::IntArrayRef(d).slice(4));
-        return once({g.dx, g.dw, g.db, Tensor(), Tensor(), Tensor(), Tensor()});
+            g.dx = shaped(g.dx, c10::IntArrayRef(d).slice(5));
+        return once({g.dx, g.dw, g.db, Tensor(), Tensor(), Tensor(), Tensor(),
+                     Tensor()});
     }
 };
 
-Tensor linear_fp8(Tensor x, Tensor w, OptTensor bias, bool relu) {
+Tensor linear_fp8(Tensor x, Tensor w, OptTensor bias, bool relu, bool exact) {
     TORCH_CHECK(w.dim() == 2, "weight must have 2 dimensions");
     if (!at::GradMode::is_enabled() ||
         !(wants_grad(x) || wants_grad(w) || wants_grad(bias)))
-        return shaped(
-            linear_fwd(as_rows(x), as_rows(w), bias, relu, false, nullptr),
-            with_last(x, w.size(0)));
-    return LinearFn::apply(x, w, bias, relu, wants_grad(x), wants_grad(w),
+        return shaped(linear_fwd(as_rows(x), as_rows(w), bias, relu, exact,
+                                 false, nullptr),
+                      with_last(x, w.size(0)));
+    return LinearFn::apply(x, w, bias, relu, exact, wants_grad(x), wants_grad(w),
                            wants_grad(bias));
 }
 
 // the same against a weight that is in 8 bits already; no gradients
 Tensor linear_fp8_serve(Tensor x0, Tensor wq, Tensor ws, int64_t block_rows,
-                        OptTensor bias, bool relu) {
+                        OptTensor bias, bool relu, bool exact) {
     TORCH_CHECK(!at::GradMode::is_enabled() ||
                     !(wants_grad(x0) || wants_grad(bias)),
                 "a weight in 8-bit blocks is for serving: pass the float "
@@ -506,7 +510,8 @@ Tensor linear_fp8_serve(Tensor x0, Tensor wq, Tensor ws, int64_t block_rows,
                      stream_of(x)),
                  "linear_fp8_blocks");
     else if (y.numel() > 0)
-        gemm(quant_rows(x).mat(), w.mat(), x.size(1), bias, relu, y, nullptr);
+        gemm(quant_rows(x).mat(), w.mat(), x.size(1), bias, relu, y, nullptr,
+             exact);
     return shaped(y, with_last(x0, w.rows));
 }
 

@@ -154,13 +154,18 @@ def dequantize_fp8_blocks(blocks: Fp8Blocks,
 
 def matmul_fp8_blocks(a: Fp8Blocks, b: Fp8Blocks,
                       bias: Optional[torch.Tensor] = None, relu: bool = False,
-                      out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """a b^T (+ bias, relu): a [M, K], b [N, K], bias [N] -> [M, N].  Sums in
+                      out_dtype: torch.dtype = torch.bfloat16,
+                      exact: bool = True) -> torch.Tensor:
+    """a b^T (+ bias, relu): a [M, K], b [N, K], bias [N] -> [M, N].  Exact
+    products (of values under 2^-126 what bfloat16 keeps of them), summed in
     fp32, rounded once to `out_dtype`.
 
-    float32: exact products (of values under 2^-126 what bfloat16 keeps of
-    them).  bfloat16, float16: products of more than a few rows may be cut at
-    2^-13 of the largest of 8 neighbours."""
+    exact=False: results in 16 bits of more than a few rows come from the
+    matrix unit's own 8-bit products, up to 1.7 times as fast.  It cuts each to
+    a multiple of 2^-13 of the largest of 8 neighbours (by their exponents), so
+    a sum is off by up to 7 x 2^-13 of its terms' magnitudes, which is all of it
+    where they cancel.  How many rows are a few goes by the sizes.  No
+    difference in float32 and on the CPU."""
     if a.cols != b.cols:
         raise RuntimeError(f"a has {a.cols} columns and b {b.cols}")
     if not a.q.is_cuda:
@@ -172,7 +177,7 @@ def matmul_fp8_blocks(a: Fp8Blocks, b: Fp8Blocks,
         return (torch.relu(z) if relu else z).to(out_dtype)
     return get_extension().fp8_blocks_matmul(
         a.q, a.scale, a.block_rows, b.q, b.scale, b.block_rows, a.cols, bias,
-        relu, out_dtype)
+        relu, out_dtype, exact)
 
 
 class _LinearFp8CpuFn(torch.autograd.Function):
@@ -201,7 +206,7 @@ class _LinearFp8CpuFn(torch.autograd.Function):
 
 
 def linear_fp8_blocks(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None,
-                      relu: bool = False) -> torch.Tensor:
+                      relu: bool = False, exact: bool = True) -> torch.Tensor:
     """x W^T + bias (relu): x [..., K], weight [N, K], bias [N] -> [..., N] in
     x's dtype.
 
@@ -212,14 +217,18 @@ def linear_fp8_blocks(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = No
     Differentiable once in x, weight and bias.  For the backward pass x is
     kept in 8 bits only; with g = Q(dz), dz = dy where the relu let through:
         dx = g Q(W)    dW = g^T Q(x)    db = sum of dz's rows
-    that is, rounding to 8 bits counts as the identity."""
+    that is, rounding to 8 bits counts as the identity.
+
+    Products of the 8-bit values are exact and summed in fp32, with and without
+    gradients alike; `exact=False` makes y and dx by matmul_fp8_blocks' faster
+    products, the relu's bits from the same sums."""
     if isinstance(weight, Fp8Blocks):
         if x.dim() > 0 and x.shape[-1] != weight.cols:
             raise RuntimeError(f"x has {x.shape[-1]} columns and weight "
                                f"{weight.cols}")
         if x.is_cuda:
             return get_extension().linear_fp8_serve(
-                x, weight.q, weight.scale, weight.block_rows, bias, relu)
+                x, weight.q, weight.scale, weight.block_rows, bias, relu, exact)
         if torch.is_grad_enabled() and (x.requires_grad or (
                 bias is not None and bias.requires_grad)):
             raise RuntimeError("a weight in 8-bit blocks is for serving: pass "
@@ -228,7 +237,7 @@ def linear_fp8_blocks(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = No
                                 relu, x.dtype)
         return out.view(*x.shape[:-1], weight.q.shape[0])
     if x.is_cuda:
-        return get_extension().linear_fp8(x, weight, bias, relu)
+        return get_extension().linear_fp8(x, weight, bias, relu, exact)
     return _LinearFp8CpuFn.apply(x, weight, bias, relu)
 
 

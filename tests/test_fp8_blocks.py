@@ -729,3 +729,86 @@ def test_no_gradient_through_blocks_cpu():
 @gpu
 def test_no_gradient_through_blocks_gpu():
     no_gradient_through("cuda")
+
+
+# -- exact products -------------------------------------------------------------
+def that_cancel(rows, cols, dtype=torch.float32):
+    """Groups of 8 columns, 1 or -1 by turns and 7 times 2^-15 in each: held in 8
+    bits exactly, and times ones the larger cancel in every partial sum of two
+    groups.  The sum, 7 cols / 8 of 2^-15, is exact in any order and in every
+    type; cut at 2^-13 of their largest, the 7 are gone."""
+    x = torch.full((rows, cols), 2.0 ** -15)
+    x[:, 0::16], x[:, 8::16] = 1.0, -1.0
+    return x.to(dtype).cuda()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,scaled", [(10, False), (300, False), (640, True),
+                                      (1500, True), (2100, True), (3700, True)])
+def test_exact_products(n, scaled, dtype):
+    """In every kind of tile, and that the other way is another."""
+    a = F.quantize_fp8_blocks(that_cancel(n, 256))
+    b = F.quantize_fp8_blocks(torch.ones(n, 256, device="cuda"), 128)
+    want = torch.full((n, n), 224 * 2.0 ** -15, dtype=dtype, device="cuda")
+    assert torch.equal(F.matmul_fp8_blocks(a, b, out_dtype=dtype), want)
+    less = F.matmul_fp8_blocks(a, b, out_dtype=dtype, exact=False)
+    assert torch.equal(less, want) != (scaled and dtype != torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("n", [10, 640, 1500, 3700])
+def test_linear_is_exact_with_and_without_gradients(n, relu):
+    x = that_cancel(n, 256, torch.bfloat16).requires_grad_()
+    w = torch.ones(n, 256, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    cols = n // 16 * 16
+    dy = torch.zeros(n, n, device="cuda", dtype=torch.bfloat16)
+    dy[:, :cols] = that_cancel(n, cols, torch.bfloat16) if cols else 0
+    y = F.linear_fp8_blocks(x, w, relu=relu)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    assert torch.equal(y, torch.full_like(y, 224 * 2.0 ** -15))
+    # 7 cols / 8 is a whole number of up to 12 bits, rounded once
+    assert torch.equal(dx, torch.full_like(dx, cols // 8 * 7 * 2.0 ** -15))
+    with torch.no_grad():
+        assert torch.equal(F.linear_fp8_blocks(x, w, relu=relu), y)
+        wb = F.quantize_fp8_blocks(w, 128)
+        assert torch.equal(F.linear_fp8_blocks(x, wb, relu=relu), y)
+    # asked for less: the same with gradients as without, relu's bits as y has them
+    y = F.linear_fp8_blocks(x, w, relu=relu, exact=False)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    with torch.no_grad():
+        assert torch.equal(F.linear_fp8_blocks(x, w, relu=relu, exact=False), y)
+        assert torch.equal(F.linear_fp8_blocks(x, wb, relu=relu, exact=False), y)
+    on = (y > 0).sum(1, keepdim=True) if relu else torch.full((n, 1), n, device="cuda")
+    assert torch.equal(dx, on.to(dx.dtype).expand_as(dx))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [
+    (16, 1024, 3136), (256, 300, 391), (288, 1024, 1300), (1037, 517, 600),
+    (1500, 1413, 300), (1665, 1280, 1100), (8200, 1056, 640), (12550, 1024, 520)])
+def test_16_bit_results_have_the_bound_of_fp32_sums(m, n, k, dtype):
+    """n 2^-24 of the magnitudes and half a step, as the module's docstring has
+    it for exact products: the product, a layer's forward pass and its dx."""
+    x = (0.25 * matrix(m, k, 1)).clamp(-8, 8).to(dtype).cuda().requires_grad_()
+    w = torch.rand(n, k, generator=torch.Generator().manual_seed(2)) - 0.5
+    w = w.to(dtype).cuda().requires_grad_()
+    dy = (0.1 * matrix(m, n, 4)).clamp(-2, 2).to(dtype).cuda()
+    xh, wh = held(x).cuda(), held(w, 128).cuda()
+    a, b = F.quantize_fp8_blocks(x), F.quantize_fp8_blocks(w, 128)
+
+    def close(got, want, terms, magnitude):
+        u = torch.finfo(dtype)
+        bound = (terms * 2.0 ** -24 * magnitude * (1 + u.eps / 2)
+                 + u.eps / 2 * want.abs() + u.smallest_normal * u.eps)
+        assert bool(((got.double() - want).abs() <= bound).all())
+
+    z, size = xh @ wh.t(), xh.abs() @ wh.abs().t()
+    close(F.matmul_fp8_blocks(a, b, out_dtype=dtype), z, k, size)
+    y = F.linear_fp8_blocks(x, w)
+    close(y, z, k, size)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    g = held(dy).cuda()
+    close(dx, g @ wh, n, g.abs() @ wh.abs())
