@@ -6,7 +6,9 @@
 //
 // The variance is the mean of squared distances from the mean, not a
 // difference of squares: rows with a large offset keep their digits.  All of
-// it in fp32, rounded once on the way out.
+// it in fp32, rounded once on the way out.  A register that adds up more than
+// some 4096 columns would not do: terms of one sign are rounded the same way
+// again and again, 2^16 of them 1e-3 off.  Longer sums go by runs.
 //
 // Both passes are bound by memory: forward reads x and writes y, backward
 // reads x and dy and writes dx.  Rows of up to 4096 columns stay in registers
@@ -126,13 +128,18 @@ DEV float wave_sum(float v) {
     v += __shfl_xor(v, 16, 64);
     return v + __shfl_xor(v, 32, 64);
 }
-// sum over 4 waves, in every thread
-DEV float group_sum(float v, float* lds) {
-    v = wave_sum(v);
-    __syncthreads();  // the last sum has been read
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+// sums over 4 waves, in every thread; `lds` is [4][2] floats
+DEV void group_sums(float& s, float& t, float* lds) {
+    s = wave_sum(s);
+    t = wave_sum(t);
+    __syncthreads();  // the last sums have been read
+    if ((threadIdx.x & 63) == 0) {
+        lds[(threadIdx.x >> 6) * 2] = s;
+        lds[(threadIdx.x >> 6) * 2 + 1] = t;
+    }
     __syncthreads();
-    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+    s = (lds[0] + lds[2]) + (lds[4] + lds[6]);
+    t = (lds[1] + lds[3]) + (lds[5] + lds[7]);
 }
 
 struct NormFwd {
@@ -255,22 +262,45 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormFwd a) {
     }
 }
 
+// Sums of two values a column over the row, in every thread.  A thread's
+// columns go in runs of 256: off by 2^-24 of its magnitude for each of 256 +
+// C / 2^16 additions at most, where one after the other would be C / 256.
+template <typename F>
+DEV void long_sums(int C, float* lds, float& s, float& t, F add) {
+    constexpr int RUN = 256 * 256;
+    s = t = 0.0f;
+    for (int c0 = threadIdx.x; c0 < C; c0 += RUN) {
+        float p = 0.0f, q = 0.0f;
+        const int end = min(c0 + RUN, C);
+        for (int c = c0; c < end; c += 256) add(c, p, q);
+        s += p;
+        t += q;
+    }
+    group_sums(s, t, lds);
+}
+
 // any number of columns, for those above 4096 and below 8: a workgroup walks
-// over its row three times
+// over its row three times.  The second walk also sums up the distances: their
+// mean is what the first one's mean is off by, and its square what the mean of
+// their squares has too much.
 template <typename T, typename W>
 __global__ __launch_bounds__(256) void norm_fwd_long_kernel(NormFwd a) {
-    __shared__ float lds[4];
+    __shared__ float lds[8];
     for (int64_t r = blockIdx.x; r < a.R; r += gridDim.x) {
         const T* x = (const T*)a.x + r * a.ldx;
-        float s = 0.0f;
-        for (int c = threadIdx.x; c < a.C; c += 256) s += to_f(x[c]);
-        const float mean = group_sum(s, lds) / a.C;
-        s = 0.0f;
-        for (int c = threadIdx.x; c < a.C; c += 256) {
-            const float d = to_f(x[c]) - mean;
-            s += d * d;
-        }
-        const float rstd = 1.0f / sqrtf(group_sum(s, lds) / a.C + a.eps);
+        float s, s2;
+        long_sums(a.C, lds, s, s2,
+                  [&](int c, float& p, float&) { p += to_f(x[c]); });
+        const float near = s / a.C;
+        long_sums(a.C, lds, s, s2, [&](int c, float& p, float& q) {
+            const float d = to_f(x[c]) - near;
+            p += d;
+            q += d * d;
+        });
+        const float off = s / a.C, mean = near + off;
+        const float var = s2 / a.C - off * off;
+        // rounding may leave less than nothing; a NaN stays one
+        const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + a.eps);
         if (a.mean && threadIdx.x == 0) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
@@ -415,19 +445,19 @@ __global__ __launch_bounds__(256, 2) void norm_bwd_kernel(NormBwd a) {
 
 template <typename T, typename W>
 __global__ __launch_bounds__(256) void norm_dx_long_kernel(NormBwd a) {
-    __shared__ float lds[4];
+    __shared__ float lds[8];
     for (int64_t r = blockIdx.x; r < a.R; r += gridDim.x) {
         const T* x = (const T*)a.x + r * a.ldx;
         const T* dy = (const T*)a.dy + r * a.lddy;
         const float mean = a.mean[r], rstd = a.rstd[r];
-        float s1 = 0.0f, s2 = 0.0f;
-        for (int c = threadIdx.x; c < a.C; c += 256) {
+        float s1, s2;
+        long_sums(a.C, lds, s1, s2, [&](int c, float& p, float& q) {
             float g = to_f(dy[c]);
             if (a.w) g *= to_f(((const W*)a.w)[c]);
-            s1 += g;
-            s2 += g * ((to_f(x[c]) - mean) * rstd);
-        }
-        const float c1 = group_sum(s1, lds) / a.C, c2 = group_sum(s2, lds) / a.C;
+            p += g;
+            q += g * ((to_f(x[c]) - mean) * rstd);
+        });
+        const float c1 = s1 / a.C, c2 = s2 / a.C;
         for (int c = threadIdx.x; c < a.C; c += 256) {
             float g = to_f(dy[c]);
             if (a.w) g *= to_f(((const W*)a.w)[c]);

@@ -381,3 +381,55 @@ def test_odd_columns(cols, types):
     got = step(x, w, b, dy)
     for name, (want, bound) in plain(x, w, b, 1e-5, dy).items():
         near(got[name], want, bound)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [4097, 32768, 100001, 2 ** 20, 2 ** 24])
+def test_long_rows_keep_their_digits(cols, dtype):
+    """Rows of one large number, of a large offset and around zero, with a
+    gradient that is one number and one of either sign.
+
+    Sums go by runs of 256 columns a thread, then of the runs, then over 256
+    threads: n = 256 + cols / 2^16 + 10 additions one behind the other, off by
+    n 2^-24 of the magnitudes.  The first mean is off by e0 = n U A, A = max |x|.
+    The distances' sum mends that up to em = U A (the mean's own rounding) +
+    n U (mean |d| + e0), and the variance is off by (n + 4) U of the mean of
+    (|d| + e0)^2, twice that for the square that is taken off, and em^2."""
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    normal = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    x = normal(3, cols)
+    x[0] = 1000.1
+    x[1] += 1000.0
+    x = x.to(dtype).requires_grad_()
+    w = (1 + 0.1 * normal(cols)).requires_grad_()
+    dy = 0.1 * normal(3, cols)
+    dy[1] = 0.1
+    dy = dy.to(dtype)
+    with torch.no_grad():
+        w[:] = torch.where(torch.arange(cols, device="cuda") % 2 == 0, w, 1.0)
+    got = {"y": F.layer_norm(x, w)}
+    got["dx"], got["dw"] = torch.autograd.grad(got["y"], (x, w), dy)
+    mean = lambda t: t.mean(1, keepdim=True)  # noqa: E731
+    n, xd, wd, dyd = 266 + cols / 2 ** 16, x.detach().double(), w.detach().double(), dy.double()
+    d = xd - mean(xd)
+    var = mean(d * d) + 1e-5
+    std = var.sqrt()
+    h = d / std
+    top = xd.abs().amax(1, keepdim=True)
+    e0 = n * U * top
+    em = U * top + n * U * (mean(d.abs()) + e0)
+    rel = ((n + 4) * U * 3 * mean((d.abs() + e0) ** 2) + em ** 2) / (2 * var) + 4 * U
+    eh = (em + U * d.abs()) / std + rel * h.abs()
+    gw = dyd * wd
+    c1, c2 = mean(gw), mean(gw * h)
+    want = {"y": (h * wd, eh * wd.abs() + 2 * U * (h * wd).abs()),
+            "dw": ((dyd * h).sum(0), (dyd.abs() * eh).sum(0)
+                   + 4 * U * (dyd * h).abs().sum(0))}
+    off = (4 * U * (gw.abs() + c1.abs() + (h * c2).abs()) + n * U * mean(gw.abs())
+           + h.abs() * (n * U * mean((gw * h).abs()) + mean(gw.abs() * eh))
+           + eh * c2.abs())
+    dx = (gw - c1 - h * c2) / std
+    want["dx"] = (dx, off / std * (1 + rel) + rel * dx.abs())
+    for name, (value, bound) in want.items():
+        near(got[name], value.cpu(), bound.cpu())
