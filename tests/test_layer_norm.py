@@ -433,3 +433,36 @@ def test_long_rows_keep_their_digits(cols, dtype):
     want["dx"] = (dx, off / std * (1 + rel) + rel * dx.abs())
     for name, (value, bound) in want.items():
         near(got[name], value.cpu(), bound.cpu())
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(2 ** 24 - 3, 8), (2 ** 24 + 5, 3),
+                                       (2 ** 21 + 1, 1032), (2 ** 22, 300)])
+def test_sums_over_many_rows(rows, cols):
+    """A gradient that is one number, and a column whose h has one sign.  A
+    register adds up 256 rows and 4 more of its last round; or 256 and then rows /
+    2^17 runs, of which 512 workgroups are left for 256 rows each; 64 parts, then
+    their runs and 16 shares.  4 waves and a rounding: 8 more."""
+    torch.manual_seed(rows)
+    x = torch.randn(rows, cols, device="cuda")
+    x[:, 0] += 50.0
+    w = torch.ones(cols, device="cuda", requires_grad=True)
+    b = torch.zeros(cols, device="cuda", requires_grad=True)
+    dy = torch.full((1, cols), 0.1, device="cuda").expand(rows, cols)
+    dw, db = torch.autograd.grad(F.layer_norm(x, w, b), (w, b), dy)
+    n = 260 + rows / 2 ** 17 + 64 + 16 + 8
+    if cols >= 8:  # parts: of 256 rows for each of a workgroup's teams
+        n = 260 + 64 + rows / 256 / (4 if cols <= 1024 else 1) / 2 ** 10 + 16 + 8
+    one = float(dy[0, 0].double())
+    assert bool(((db.double() - one * rows).abs() <= n * U * one * rows).all())
+    var, mean = torch.var_mean(x.double(), 1, unbiased=False)
+    std = (var + 1e-5).sqrt()
+    for c in (0, 1, cols - 1):
+        h = (x[:, c].double() - mean) / std
+        top = x.abs().amax(1).double()
+        eh = (cols + 4) * U * top / std + (cols + 8) * U * h.abs()
+        bound = (n * U * h.abs() + eh).sum() * one
+        if c == 0:  # h is off by some 2^-24 either way, row by row: of 2^21 rows
+            # and more 1 % of the worst case is far from what is left
+            bound = (n * U * h.abs() + 0.01 * eh).sum() * one
+        assert float((dw[c].double() - one * h.sum()).abs()) <= float(bound)
