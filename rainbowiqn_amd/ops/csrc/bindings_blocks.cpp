@@ -152,10 +152,15 @@ Mat mat_at(uint8_t* base, std::pair<int64_t, int64_t> at, int64_t rows,
 
 // Groups of rows for a quantisation that also sums up the columns: every group
 // leaves a row of partial sums to be added up, and 1024 workgroups in all fill
-// the card and keep those few.
+// the card and keep those few.  More where a lane's register would add up over
+// 256 rows, as far as a grid goes.
 int sum_groups(int64_t R, int64_t C) {
     const int64_t nb = blocks_of(C), strips = nb >= 4 ? (nb + 3) / 4 : nb;
-    return quant_groups(R, C, std::max<int64_t>(1, 1024 / strips));
+    const int64_t run = 256 * (nb >= 4 ? 4 : 16);  // a group's rows
+    return quant_groups(
+        R, C,
+        std::min<int64_t>(65535, std::max<int64_t>({1, 1024 / strips,
+                                                    (R + run - 1) / run})));
 }
 
 // scale per 1 x 128 block; with `mask` values whose bit is clear count as

@@ -229,7 +229,9 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(
 }
 
 // out[c] = sum over G rows of part[g][c]; 64 columns and 16 shares of the rows
-// a workgroup, so that no load waits for another
+// a workgroup, so that no load waits for another.  A share goes in runs of 64
+// rows, then the runs: one register over thousands of terms of one sign is 1e-5
+// and more off.
 template <typename T>
 __global__ __launch_bounds__(1024) void column_sum_kernel(
     const float* __restrict__ part, T* __restrict__ out, int G, int C) {
@@ -237,8 +239,13 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(
     const int c = blockIdx.x * 64 + (threadIdx.x & 63), g0 = threadIdx.x >> 6;
     float t = 0.0f;
     if (c < C) {
-        #pragma unroll 8
-        for (int g = g0; g < G; g += 16) t += part[(int64_t)g * C + c];
+        for (int from = g0; from < G; from += 16 * 64) {
+            float p = 0.0f;
+            const int end = min(from + 16 * 64, G);
+            #pragma unroll 8
+            for (int g = from; g < end; g += 16) p += part[(int64_t)g * C + c];
+            t += p;
+        }
     }
     red[g0][threadIdx.x & 63] = t;
     __syncthreads();

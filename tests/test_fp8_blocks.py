@@ -812,3 +812,24 @@ def test_16_bit_results_have_the_bound_of_fp32_sums(m, n, k, dtype):
     (dx,) = torch.autograd.grad(y, x, dy)
     g = held(dy).cuda()
     close(dx, g @ wh, n, g.abs() @ wh.abs())
+
+
+@gpu
+@pytest.mark.parametrize("rows,outs", [(2 ** 27 - 5, 1), (2 ** 26 + 3, 130)])
+def test_bias_gradient_over_many_rows(rows, outs):
+    """Of a gradient that is one number.  A lane adds up 256 rows (as many as
+    65535 groups leave it, 64 or 16 rows a time) and 1 of its last round, 4 waves
+    and 4 rows of a wave, then runs of 64 parts, the runs and 16 shares."""
+    x = torch.ones(rows, 1, device="cuda", dtype=torch.bfloat16)
+    w = torch.ones(outs, 1, device="cuda", dtype=torch.bfloat16)
+    b = torch.zeros(outs, device="cuda", requires_grad=True)
+    # the type of the result is x's, so the gradient of 24 bits goes by float32
+    x, w = (x.float(), w.float()) if outs == 1 else (x, w)
+    y = F.linear_fp8_blocks(x, w, b)
+    dy = torch.full((1, outs), 0.1, device="cuda").to(y.dtype).expand(rows, outs)
+    (db,) = torch.autograd.grad(y, b, dy)
+    lanes = max(256, -(-rows // (65535 * 16)))
+    groups = -(-rows // (16 * lanes))
+    n = lanes + 1 + 8 + 64 + groups / 2 ** 10 + 16
+    want = float(dy[0, 0].double()) * rows
+    assert bool(((db.double() - want).abs() <= n * 2.0 ** -24 * want).all())
