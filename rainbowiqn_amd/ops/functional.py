@@ -165,7 +165,13 @@ def matmul_fp8_blocks(a: Fp8Blocks, b: Fp8Blocks,
     a multiple of 2^-13 of the largest of 8 neighbours (by their exponents), so
     a sum is off by up to 7 x 2^-13 of its terms' magnitudes, which is all of it
     where they cancel.  How many rows are a few goes by the sizes.  No
-    difference in float32 and on the CPU."""
+    difference in float32 and on the CPU.
+
+    Has no gradients: a bias that wants one is refused while they are
+    recorded."""
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("a product of 8-bit blocks has no gradients: pass "
+                           "bias.detach(), or train with linear_fp8_blocks")
     if a.cols != b.cols:
         raise RuntimeError(f"a has {a.cols} columns and b {b.cols}")
     if not a.q.is_cuda:

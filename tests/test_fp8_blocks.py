@@ -833,3 +833,24 @@ def test_bias_gradient_over_many_rows(rows, outs):
     n = lanes + 1 + 8 + 64 + groups / 2 ** 10 + 16
     want = float(dy[0, 0].double()) * rows
     assert bool(((db.double() - want).abs() <= n * 2.0 ** -24 * want).all())
+
+
+def bias_that_wants_a_gradient(device):
+    """Refused instead of lost."""
+    a = F.quantize_fp8_blocks(matrix(5, 200, 1, device=device))
+    bias = torch.ones(5, device=device, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        F.matmul_fp8_blocks(a, a, bias)
+    want = F.matmul_fp8_blocks(a, a, bias.detach())
+    assert not want.requires_grad
+    with torch.no_grad():
+        assert torch.equal(F.matmul_fp8_blocks(a, a, bias), want)
+
+
+def test_bias_that_wants_a_gradient_cpu():
+    bias_that_wants_a_gradient("cpu")
+
+
+@gpu
+def test_bias_that_wants_a_gradient_gpu():
+    bias_that_wants_a_gradient("cuda")
