@@ -35,6 +35,16 @@ int type_code(at::ScalarType t, const char* name) {
     }
 }
 
+// What an operator is handed: forward-mode derivatives are not there, and a
+// tangent that the kernels cannot see would count as zero.
+void check_given(const Tensor& t) {
+    TORCH_CHECK(!t._fw_grad(0).defined(),
+                "this operator has no forward-mode derivatives");
+}
+void check_given(const OptTensor& t) {
+    if (t) check_given(*t);
+}
+
 // a matrix whose rows are contiguous and any stride apart
 void check_rows(const Tensor& x, const char* name) {
     TORCH_CHECK(x.is_cuda(), name, " must be on GPU");
@@ -240,6 +250,7 @@ Tensor fp8_blocks_matmul(Tensor aq, Tensor as, int64_t a_block_rows, Tensor bq,
                          Tensor bs, int64_t b_block_rows, int64_t cols,
                          OptTensor bias, bool relu, at::ScalarType dtype,
                          bool exact) {
+    check_given(bias);
     Blocks a = check_blocks(aq, as, cols, a_block_rows, "a");
     Blocks b = check_blocks(bq, bs, cols, b_block_rows, "b");
     TORCH_CHECK(aq.device() == bq.device(), "a and b must be on one GPU");
@@ -477,6 +488,9 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
 };
 
 Tensor linear_fp8(Tensor x, Tensor w, OptTensor bias, bool relu, bool exact) {
+    check_given(x);
+    check_given(w);
+    check_given(bias);
     TORCH_CHECK(w.dim() == 2, "weight must have 2 dimensions");
     if (!at::GradMode::is_enabled() ||
         !(wants_grad(x) || wants_grad(w) || wants_grad(bias)))
@@ -494,6 +508,8 @@ Tensor linear_fp8_serve(Tensor x0, Tensor wq, Tensor ws, int64_t block_rows,
                     !(wants_grad(x0) || wants_grad(bias)),
                 "a weight in 8-bit blocks is for serving: pass the float "
                 "weight where gradients are wanted");
+    check_given(x0);
+    check_given(bias);
     const Tensor x = as_rows(x0);
     check_rows(x, "x");
     Blocks w = check_blocks(wq, ws, x.size(1), block_rows, "weight");
@@ -621,6 +637,9 @@ class NormFn : public torch::autograd::Function<NormFn> {
 };
 
 Tensor layer_norm(Tensor x, OptTensor w, OptTensor b, double eps) {
+    check_given(x);
+    check_given(w);
+    check_given(b);
     if (!at::GradMode::is_enabled() ||
         !(wants_grad(x) || wants_grad(w) || wants_grad(b)))
         return shaped(norm_fwd(as_rows(x), w, b, eps, nullptr), x.sizes());

@@ -8,6 +8,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import get_extension, torch_ref
@@ -86,7 +87,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
 
     x: float32, bfloat16 or float16, any strides (rows that are not contiguous
     are copied first); weight and bias [C], contiguous, either or both left
-    out, in x's dtype or float32.  Differentiable once in x, weight and bias.
+    out, in x's dtype or float32.  Differentiable once in x, weight and bias, in
+    reverse mode; forward-mode derivatives on the CPU alone.
     GPU: one kernel forward, two backward; CPU: torch_ref, same semantics.
     """
     if not x.is_cuda:
@@ -178,6 +180,7 @@ def matmul_fp8_blocks(a: Fp8Blocks, b: Fp8Blocks,
         _check_blocks(a, "a")
         _check_blocks(b, "b")
         _check_bias(bias, b.q.shape[0])
+        _check_tangents(bias)
         z = (dequantize_fp8_blocks(a) @ dequantize_fp8_blocks(b).t())
         z = z if bias is None else z + bias.float()
         return (torch.relu(z) if relu else z).to(out_dtype)
@@ -220,8 +223,9 @@ def linear_fp8_blocks(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = No
     and the weight per 128 x 128.  `weight` is a float matrix, or Fp8Blocks
     that quantize_fp8_blocks(w, 128) laid out once (for serving; no gradients).
 
-    Differentiable once in x, weight and bias.  For the backward pass x is
-    kept in 8 bits only; with g = Q(dz), dz = dy where the relu let through:
+    Differentiable once in x, weight and bias, in reverse mode.  For the
+    backward pass x is kept in 8 bits only; with g = Q(dz), dz = dy where the
+    relu let through:
         dx = g Q(W)    dW = g^T Q(x)    db = sum of dz's rows
     that is, rounding to 8 bits counts as the identity.
 
@@ -239,6 +243,7 @@ def linear_fp8_blocks(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = No
                 bias is not None and bias.requires_grad)):
             raise RuntimeError("a weight in 8-bit blocks is for serving: pass "
                                "the float weight where gradients are wanted")
+        _check_tangents(x, bias)
         out = matmul_fp8_blocks(quantize_fp8_blocks(_rows(x)), weight, bias,
                                 relu, x.dtype)
         return out.view(*x.shape[:-1], weight.q.shape[0])
@@ -271,6 +276,12 @@ def _check_matrix(x, name):
 def _check_bias(bias, n):
     if bias is not None and (bias.dim() != 1 or bias.shape[0] != n):
         raise RuntimeError(f"bias must have {n} elements in 1 dimension")
+
+
+def _check_tangents(*tensors):
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("this operator has no forward-mode derivatives")
 
 
 def _check_norm(x, weight, bias, eps):

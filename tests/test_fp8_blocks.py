@@ -854,3 +854,37 @@ def test_bias_that_wants_a_gradient_cpu():
 @gpu
 def test_bias_that_wants_a_gradient_gpu():
     bias_that_wants_a_gradient("cuda")
+
+
+def tangents(device):
+    """A forward-mode derivative is refused instead of lost."""
+    from torch.autograd import forward_ad
+
+    x, w = matrix(5, 200, 1, device=device), matrix(7, 200, 2, device=device)
+    b = torch.ones(7, device=device)
+    xb, wb = F.quantize_fp8_blocks(x), F.quantize_fp8_blocks(w, 128)
+    calls = [lambda d: F.linear_fp8_blocks(d(x), w, b),
+             lambda d: F.linear_fp8_blocks(x, d(w), b),
+             lambda d: F.linear_fp8_blocks(x, w, d(b)),
+             lambda d: F.linear_fp8_blocks(d(x), wb, b),
+             lambda d: F.linear_fp8_blocks(x, wb, d(b)),
+             lambda d: F.matmul_fp8_blocks(xb, wb, d(b))]
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        of_leaf = lambda t: dual(t.clone().requires_grad_())  # noqa: E731
+        for i, call in enumerate(calls):
+            for d in (dual, of_leaf):
+                for mode in (torch.no_grad, torch.enable_grad):
+                    with mode(), pytest.raises(RuntimeError):
+                        call(d)
+                        pytest.fail(f"call {i} was not refused")
+            call(lambda t: t)  # without one, inside the level
+
+
+def test_tangents_cpu():
+    tangents("cpu")
+
+
+@gpu
+def test_tangents_gpu():
+    tangents("cuda")

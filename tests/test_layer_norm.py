@@ -466,3 +466,43 @@ def test_sums_over_many_rows(rows, cols):
             # and more 1 % of the worst case is far from what is left
             bound = (n * U * h.abs() + 0.01 * eh).sum() * one
         assert float((dw[c].double() - one * h.sum()).abs()) <= float(bound)
+
+
+def duals(x, w, b):
+    from torch.autograd import forward_ad
+
+    for i in range(3):
+        args = [x, w, b]
+        args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+        yield i, F.layer_norm, args
+
+
+@gpu
+@pytest.mark.parametrize("cols", [30, 5000])
+def test_tangents_are_refused(cols):
+    """Instead of a result without one, which would count as zero."""
+    from torch.autograd import forward_ad
+
+    x, w, b, _ = inputs(4, cols, torch.float32, torch.float32, "cuda")
+    for leaves in ((x, w, b), tuple(t.detach() for t in (x, w, b))):
+        with forward_ad.dual_level():
+            for _, call, args in duals(*leaves):
+                for mode in (torch.no_grad, torch.enable_grad):
+                    with mode(), pytest.raises(RuntimeError):
+                        call(*args)
+            F.layer_norm(*leaves)
+
+
+def test_tangents_cpu():
+    """There the derivative in x's, weight's and bias's direction is right."""
+    from torch.autograd import forward_ad
+
+    x, w, b, _ = (t.detach() for t in inputs(4, 30, torch.float32, torch.float32, "cpu"))
+    d = x.double() - x.double().mean(1, keepdim=True)
+    h = d / ((d * d).mean(1, keepdim=True) + 1e-5).sqrt()
+    # x moved by one number: y stays; weight by 1: h; bias by 1: 1
+    want = [torch.zeros_like(h), h, torch.ones_like(h)]
+    with forward_ad.dual_level():
+        for i, call, args in duals(x, w, b):
+            got = forward_ad.unpack_dual(call(*args)).tangent
+            assert bool(((got.expand_as(h).double() - want[i]).abs() <= 1e-5).all())
