@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <tuple>
 
 #include "riqn_kernels.h"
@@ -33,6 +34,13 @@ int type_code(at::ScalarType t, const char* name) {
             TORCH_CHECK(false, name, " must be float32, bfloat16 or float16, got ",
                         at::toString(t));
     }
+}
+
+// A tracer sees the allocations of a call and none of its kernels: what it
+// records would return memory that nobody wrote.
+void check_call() {
+    TORCH_CHECK(!torch::jit::tracer::isTracing(),
+                "this operator's GPU kernels cannot be traced");
 }
 
 // What an operator is handed: forward-mode derivatives are not there, and a
@@ -221,6 +229,7 @@ void gemm(const Mat& a, const Mat& b, int64_t K, const OptTensor& bias,
 }
 
 std::tuple<Tensor, Tensor> fp8_blocks_quant(Tensor x, int64_t block_rows) {
+    check_call();
     check_rows(x, "x");
     TORCH_CHECK(x.size(1) >= 1, "x must have at least one column");
     TORCH_CHECK(block_rows == 1 || block_rows == 128, "block_rows must be 1 or 128");
@@ -234,6 +243,7 @@ std::tuple<Tensor, Tensor> fp8_blocks_quant(Tensor x, int64_t block_rows) {
 
 Tensor fp8_blocks_dequant(Tensor q, Tensor scale, int64_t cols,
                           int64_t block_rows, at::ScalarType dtype) {
+    check_call();
     Blocks b = check_blocks(q, scale, cols, block_rows, "blocks");
     const int type = type_code(dtype, "dtype");
     c10::cuda::CUDAGuard guard(q.device());
@@ -250,6 +260,7 @@ Tensor fp8_blocks_matmul(Tensor aq, Tensor as, int64_t a_block_rows, Tensor bq,
                          Tensor bs, int64_t b_block_rows, int64_t cols,
                          OptTensor bias, bool relu, at::ScalarType dtype,
                          bool exact) {
+    check_call();
     check_given(bias);
     Blocks a = check_blocks(aq, as, cols, a_block_rows, "a");
     Blocks b = check_blocks(bq, bs, cols, b_block_rows, "b");
@@ -488,6 +499,7 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
 };
 
 Tensor linear_fp8(Tensor x, Tensor w, OptTensor bias, bool relu, bool exact) {
+    check_call();
     check_given(x);
     check_given(w);
     check_given(bias);
@@ -508,6 +520,7 @@ Tensor linear_fp8_serve(Tensor x0, Tensor wq, Tensor ws, int64_t block_rows,
                     !(wants_grad(x0) || wants_grad(bias)),
                 "a weight in 8-bit blocks is for serving: pass the float "
                 "weight where gradients are wanted");
+    check_call();
     check_given(x0);
     check_given(bias);
     const Tensor x = as_rows(x0);
@@ -637,6 +650,7 @@ class NormFn : public torch::autograd::Function<NormFn> {
 };
 
 Tensor layer_norm(Tensor x, OptTensor w, OptTensor b, double eps) {
+    check_call();
     check_given(x);
     check_given(w);
     check_given(b);

@@ -89,7 +89,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     are copied first); weight and bias [C], contiguous, either or both left
     out, in x's dtype or float32.  Differentiable once in x, weight and bias, in
     reverse mode; forward-mode derivatives on the CPU alone.
-    GPU: one kernel forward, two backward; CPU: torch_ref, same semantics.
+    GPU: one kernel forward, two backward, refused under torch.jit.trace, as are
+    the operators below; CPU: torch_ref, same semantics.
     """
     if not x.is_cuda:
         _check_norm(x, weight, bias, eps)

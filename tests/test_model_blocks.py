@@ -233,3 +233,23 @@ def test_captured_loss_replays():
         assert torch.equal(per, want_per)
         # added up by atomics: 32 terms of one sign in any order
         assert abs(float(loss - want)) <= 64 * 2.0 ** -24 * float(want)
+
+
+@gpu
+def test_tracing_is_refused():
+    """Instead of a record that holds the allocations and no kernel."""
+    x = torch.randn(5, 200, device="cuda")
+    w = torch.randn(7, 200, device="cuda")
+    xb, wb = F.quantize_fp8_blocks(x), F.quantize_fp8_blocks(w, 128)
+    for call in (lambda z: F.layer_norm(z), lambda z: F.linear_fp8_blocks(z, w),
+                 lambda z: F.linear_fp8_blocks(z.detach(), wb),
+                 lambda z: F.quantize_fp8_blocks(z).q,
+                 lambda z: F.dequantize_fp8_blocks(xb) + z,
+                 lambda z: F.matmul_fp8_blocks(xb, xb) + z[:, :5]):
+        for t in (x, x.clone().requires_grad_()):
+            call(t)
+            with pytest.raises(RuntimeError, match="traced"):
+                torch.jit.trace(call, (t,), check_trace=False)
+    net, h = head_and_input("cuda", torch.float32, 3)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda z: net.head(z), (h,), check_trace=False)
