@@ -43,9 +43,29 @@ void check_call() {
                 "this operator's GPU kernels cannot be traced");
 }
 
+// The kernels read and write memory.  A tensor that stands for others (a
+// subclass that holds them, a transform's), for shapes alone or for zeros has
+// none, and its address is null.
+void check_memory(const Tensor& t) {
+    using c10::DispatchKey;
+    TORCH_CHECK(t.has_storage() &&
+                    !t.key_set().has_any(c10::DispatchKeySet(
+                        {DispatchKey::Python, DispatchKey::Functionalize,
+                         DispatchKey::ZeroTensor})),
+                "a tensor without memory of its own is not for this operator");
+}
+
+// torch's allocator, unless a mode hands out something else in its place
+Tensor fresh(c10::IntArrayRef sizes, const at::TensorOptions& options) {
+    Tensor t = torch::empty(sizes, options);
+    check_memory(t);
+    return t;
+}
+
 // What an operator is handed: forward-mode derivatives are not there, and a
 // tangent that the kernels cannot see would count as zero.
 void check_given(const Tensor& t) {
+    check_memory(t);
     TORCH_CHECK(!t._fw_grad(0).defined(),
                 "this operator has no forward-mode derivatives");
 }
@@ -92,6 +112,8 @@ struct Blocks {
 // checks what the kernels take for granted about a matrix given from outside
 Blocks check_blocks(const Tensor& q, const Tensor& scale, int64_t cols,
                     int64_t block_rows, const char* name) {
+    check_memory(q);
+    check_memory(scale);
     TORCH_CHECK(q.is_cuda() && scale.device() == q.device(), name,
                 ": q and scale must be on one GPU");
     TORCH_CHECK(q.scalar_type() == torch::kUInt8 &&
@@ -133,9 +155,9 @@ int row_groups(int64_t rows, int64_t rows_per_pass, int64_t most) {
 Blocks new_blocks(const Tensor& like, int64_t R, int64_t C,
                   int64_t block_rows) {
     const int64_t nb = blocks_of(C);
-    return {torch::empty({R, nb * 128}, bytes_on(like)),
-            torch::empty({block_rows == 1 ? R : blocks_of(R), padded4(nb)},
-                         bytes_on(like)),
+    return {fresh({R, nb * 128}, bytes_on(like)),
+            fresh({block_rows == 1 ? R : blocks_of(R), padded4(nb)},
+                  bytes_on(like)),
             R, block_rows};
 }
 
@@ -230,6 +252,7 @@ void gemm(const Mat& a, const Mat& b, int64_t K, const OptTensor& bias,
 
 std::tuple<Tensor, Tensor> fp8_blocks_quant(Tensor x, int64_t block_rows) {
     check_call();
+    check_memory(x);
     check_rows(x, "x");
     TORCH_CHECK(x.size(1) >= 1, "x must have at least one column");
     TORCH_CHECK(block_rows == 1 || block_rows == 128, "block_rows must be 1 or 128");
@@ -247,7 +270,7 @@ Tensor fp8_blocks_dequant(Tensor q, Tensor scale, int64_t cols,
     Blocks b = check_blocks(q, scale, cols, block_rows, "blocks");
     const int type = type_code(dtype, "dtype");
     c10::cuda::CUDAGuard guard(q.device());
-    Tensor out = torch::empty({b.rows, cols}, q.options().dtype(dtype));
+    Tensor out = fresh({b.rows, cols}, q.options().dtype(dtype));
     if (b.rows == 0) return out;
     launched(riqn_fp8_dequant(q.data_ptr<uint8_t>(), scale.data_ptr<uint8_t>(),
                               out.data_ptr(), type, (int)b.rows, (int)cols,
@@ -271,7 +294,7 @@ Tensor fp8_blocks_matmul(Tensor aq, Tensor as, int64_t a_block_rows, Tensor bq,
     }
     type_code(dtype, "out_dtype");
     c10::cuda::CUDAGuard guard(aq.device());
-    Tensor c = torch::empty({a.rows, b.rows}, aq.options().dtype(dtype));
+    Tensor c = fresh({a.rows, b.rows}, aq.options().dtype(dtype));
     if (c.numel() == 0) return c;
     gemm(a.mat(), b.mat(), cols, bias, relu, c, nullptr, exact);
     return c;
@@ -369,15 +392,15 @@ Tensor linear_fwd(const Tensor& x, const Tensor& w, const OptTensor& bias,
     check_tiles(w);
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t M = x.size(0), N = w.size(0), K = x.size(1);
-    Tensor y = torch::empty({M, N}, x.options());
+    Tensor y = fresh({M, N}, x.options());
     if (M == 0 && !keep) return y;
     const Kept at(M, N, K, need_dx, relu && keep);
     Carve c;
     const auto w_at = c.matrix(N, K, 128);
     const int64_t x_at = c.take(keep ? 0 : at.size);
-    Tensor work = torch::empty({c.size}, bytes_on(x));
+    Tensor work = fresh({c.size}, bytes_on(x));
     auto* const base = work.data_ptr<uint8_t>();
-    if (keep) *keep = torch::empty({at.size}, bytes_on(x));
+    if (keep) *keep = fresh({at.size}, bytes_on(x));
     auto* const kept = keep ? keep->data_ptr<uint8_t>() : base + x_at;
     const Mat xq = mat_at(kept, at.x, M, 1), wq = mat_at(base, w_at, N, 128);
     const Mat wt = need_dx ? mat_at(kept, at.wt, K, 128) : Mat{};
@@ -414,12 +437,13 @@ LinearGrads linear_bwd(const Tensor& dy, const Tensor& keep, int64_t K, bool rel
     type_code(dy.scalar_type(), "dy");
     const int64_t M = dy.size(0), N = dy.size(1);
     const Kept at(M, N, K, dx_type.has_value(), relu);
-    TORCH_CHECK(keep.size(0) == at.size, "dy does not have the result's rows");
+    TORCH_CHECK(keep.device() == dy.device() && keep.size(0) == at.size,
+                "dy does not have the result's rows or device");
     c10::cuda::CUDAGuard guard(dy.device());
     LinearGrads o;
-    if (dx_type) o.dx = torch::empty({M, K}, dy.options().dtype(*dx_type));
-    if (dw_type) o.dw = torch::empty({N, K}, dy.options().dtype(*dw_type));
-    if (db_type) o.db = torch::empty({N}, dy.options().dtype(*db_type));
+    if (dx_type) o.dx = fresh({M, K}, dy.options().dtype(*dx_type));
+    if (dw_type) o.dw = fresh({N, K}, dy.options().dtype(*dw_type));
+    if (db_type) o.db = fresh({N}, dy.options().dtype(*db_type));
     if (M == 0) {
         if (dw_type) o.dw.zero_();
         if (db_type) o.db.zero_();
@@ -435,7 +459,7 @@ LinearGrads linear_bwd(const Tensor& dy, const Tensor& keep, int64_t K, bool rel
     const auto g_at = c.matrix(M, N, 1);
     const int64_t sum_at = c.take(db_type ? groups * N * 4 : 0);
     const int64_t part_at = c.take(dw_type && shares > 1 ? shares * N * K * 4 : 0);
-    Tensor work = torch::empty({c.size}, bytes_on(dy));
+    Tensor work = fresh({c.size}, bytes_on(dy));
     auto* const base = work.data_ptr<uint8_t>();
     auto* const kept = keep.data_ptr<uint8_t>();
     const Mat g = mat_at(base, g_at, M, 1), x = mat_at(kept, at.x, M, 1);
@@ -482,6 +506,7 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
     static torch::autograd::variable_list backward(
         torch::autograd::AutogradContext* ctx,
         torch::autograd::variable_list dy) {
+        check_given(dy[0]);
         check_capture(dy[0]);
         const auto v = ctx->get_saved_variables();
         const auto d = ctx->saved_data["all"].toIntVector();
@@ -533,7 +558,7 @@ Tensor linear_fp8_serve(Tensor x0, Tensor wq, Tensor ws, int64_t block_rows,
     }
     type_code(x.scalar_type(), "x");
     c10::cuda::CUDAGuard guard(x.device());
-    Tensor y = torch::empty({x.size(0), w.rows}, x.options());
+    Tensor y = fresh({x.size(0), w.rows}, x.options());
     if (y.numel() > 0 && riqn_fp8_few(x.size(0), (int)x.size(1)))
         launched(riqn_fp8_gemm_from(
                      x.data_ptr(), type_code(x.scalar_type(), "x"), x.stride(0),
@@ -573,10 +598,10 @@ Tensor norm_fwd(const Tensor& x, const OptTensor& w, const OptTensor& b,
     TORCH_CHECK(eps >= 0.0, "eps must not be negative");
     const int wt = norm_weights(x, w, b);
     c10::cuda::CUDAGuard guard(x.device());
-    Tensor y = torch::empty({x.size(0), x.size(1)}, x.options());
+    Tensor y = fresh({x.size(0), x.size(1)}, x.options());
     float* mean = nullptr;
     if (stats) {
-        *stats = torch::empty({2 * x.size(0)}, floats_on(x));
+        *stats = fresh({2 * x.size(0)}, floats_on(x));
         mean = stats->data_ptr<float>();
     }
     if (x.size(0) > 0)
@@ -608,9 +633,14 @@ class NormFn : public torch::autograd::Function<NormFn> {
     static torch::autograd::variable_list backward(
         torch::autograd::AutogradContext* ctx,
         torch::autograd::variable_list grad) {
+        check_given(grad[0]);
         check_capture(grad[0]);
         const auto v = ctx->get_saved_variables();
         const Tensor &x = v[0], &w = v[1];
+        check_rows(x, "x");
+        TORCH_CHECK(v[2].device() == x.device() &&
+                        (!w.defined() || w.device() == x.device()),
+                    "what was kept must be on one GPU");
         const float* const mean = v[2].data_ptr<float>();
         const auto d = ctx->saved_data["all"].toIntVector();
         const int64_t need = d[0];
@@ -622,16 +652,16 @@ class NormFn : public torch::autograd::Function<NormFn> {
         const int64_t R = x.size(0), C = x.size(1);
         c10::cuda::CUDAGuard guard(x.device());
         Tensor dx, dw, db;
-        if (need & 1) dx = torch::empty({R, C}, x.options());
-        if (need & 2) dw = torch::empty({C}, x.options().dtype(w_type));
-        if (need & 4) db = torch::empty({C}, x.options().dtype(w_type));
+        if (need & 1) dx = fresh({R, C}, x.options());
+        if (need & 2) dw = fresh({C}, x.options().dtype(w_type));
+        if (need & 4) db = fresh({C}, x.options().dtype(w_type));
         if (R == 0) {
             if (dw.defined()) dw.zero_();
             if (db.defined()) db.zero_();
         } else {
             const int groups = riqn_norm_groups((int)R, (int)C);
             Tensor part;
-            if (need & 6) part = torch::empty({groups, 2, C}, floats_on(x));
+            if (need & 6) part = fresh({groups, 2, C}, floats_on(x));
             launched(riqn_norm_bwd(
                          dy.data_ptr(), x.data_ptr(),
                          type_code(x.scalar_type(), "x"), dy.stride(0),

@@ -253,3 +253,59 @@ def test_tracing_is_refused():
     net, h = head_and_input("cuda", torch.float32, 3)
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda z: net.head(z), (h,), check_trace=False)
+
+
+class Holds(torch.Tensor):
+    """A subclass that holds a tensor and has no memory of its own."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(
+            cls, t.shape, dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(str(func))
+
+
+@gpu
+def test_tensors_without_memory_are_refused():
+    """Their address is null."""
+    from torch._subclasses import FakeTensorMode
+
+    x, w = torch.randn(5, 200, device="cuda"), torch.randn(7, 200, device="cuda")
+    b, n = torch.randn(7, device="cuda"), torch.randn(200, device="cuda")
+    xb, wb = F.quantize_fp8_blocks(x), F.quantize_fp8_blocks(w, 128)
+    whole = [lambda x: F.layer_norm(x, n, n), lambda x: F.linear_fp8_blocks(x, w, b),
+             lambda x: F.linear_fp8_blocks(x, wb, b),
+             lambda x: F.quantize_fp8_blocks(x, 128)]
+    parts = [(n, lambda t: F.layer_norm(x, t, n)), (n, lambda t: F.layer_norm(x, n, t)),
+             (w, lambda t: F.linear_fp8_blocks(x, t, b)),
+             (b, lambda t: F.linear_fp8_blocks(x, w, t)),
+             (b, lambda t: F.linear_fp8_blocks(x, wb, t)),
+             (wb.q, lambda t: F.linear_fp8_blocks(x, wb._replace(q=t))),
+             (wb.scale, lambda t: F.linear_fp8_blocks(x, wb._replace(scale=t))),
+             (xb.q, lambda t: F.dequantize_fp8_blocks(xb._replace(q=t))),
+             (xb.scale, lambda t: F.matmul_fp8_blocks(xb._replace(scale=t), wb)),
+             (wb.q, lambda t: F.matmul_fp8_blocks(xb, wb._replace(q=t))),
+             (b, lambda t: F.matmul_fp8_blocks(xb, wb, t))]
+    parts += [(x, call) for call in whole]
+    for t, call in parts:
+        with pytest.raises(RuntimeError):
+            call(Holds(t))
+        with pytest.raises(RuntimeError):
+            call(torch._efficientzerotensor(t.shape, dtype=t.dtype, device="cuda"))
+        with pytest.raises(RuntimeError):
+            torch.func.functionalize(call)(t)
+        if t.is_floating_point():
+            with pytest.raises(RuntimeError):
+                torch.func.vmap(call)(t.expand(2, *t.shape))
+            with pytest.raises(RuntimeError):
+                torch.func.grad(lambda t: call(t).sum())(t)
+            with pytest.raises(RuntimeError):
+                torch.func.jvp(call, (t,), (t,))
+        # real arguments, results that are shapes alone
+        with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(RuntimeError):
+            call(t)
+        call(t)
+    torch.cuda.synchronize()
