@@ -88,7 +88,8 @@ void check_vector(const Tensor& v, int64_t n, const Tensor& like,
     TORCH_CHECK(v.device() == like.device(), name, " must be on ", like.device());
     TORCH_CHECK(v.dim() == 1 && v.size(0) == n, name, " must have ", n,
                 " elements in 1 dimension");
-    TORCH_CHECK(v.is_contiguous(), name, " must be contiguous");
+    TORCH_CHECK(v.is_contiguous() && !v.is_neg(), name,
+                " must be contiguous, and no negated view");
 }
 
 int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
@@ -114,6 +115,8 @@ Blocks check_blocks(const Tensor& q, const Tensor& scale, int64_t cols,
                     int64_t block_rows, const char* name) {
     check_memory(q);
     check_memory(scale);
+    TORCH_CHECK(!q.is_neg() && !scale.is_neg(), name,
+                ": q and scale must be no negated views");
     TORCH_CHECK(q.is_cuda() && scale.device() == q.device(), name,
                 ": q and scale must be on one GPU");
     TORCH_CHECK(q.scalar_type() == torch::kUInt8 &&
@@ -253,6 +256,7 @@ void gemm(const Mat& a, const Mat& b, int64_t K, const OptTensor& bias,
 std::tuple<Tensor, Tensor> fp8_blocks_quant(Tensor x, int64_t block_rows) {
     check_call();
     check_memory(x);
+    x = x.resolve_neg();
     check_rows(x, "x");
     TORCH_CHECK(x.size(1) >= 1, "x must have at least one column");
     TORCH_CHECK(block_rows == 1 || block_rows == 128, "block_rows must be 1 or 128");
@@ -302,11 +306,11 @@ Tensor fp8_blocks_matmul(Tensor aq, Tensor as, int64_t a_block_rows, Tensor bq,
 
 // x [..., C] as a matrix of contiguous rows, copied only where it must
 Tensor as_rows(const Tensor& x) {
-    Tensor r = x;
+    Tensor r = x.resolve_neg();  // a view that negates is negated here
     if (x.dim() != 2) {
         TORCH_CHECK(x.dim() > 0, "a matrix or a vector is wanted, not a number");
         const int64_t c = x.size(-1);
-        r = x.reshape({x.numel() / std::max<int64_t>(1, c), c});
+        r = r.reshape({x.numel() / std::max<int64_t>(1, c), c});
     }
     return r.size(1) <= 1 || r.stride(1) == 1 ? r : r.contiguous();
 }

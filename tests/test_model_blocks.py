@@ -309,3 +309,33 @@ def test_tensors_without_memory_are_refused():
             call(t)
         call(t)
     torch.cuda.synchronize()
+
+
+@gpu
+@pytest.mark.parametrize("cols", [1, 200])
+def test_negated_views(cols):
+    """A view that negates has the memory of what it negates."""
+    x = torch.randn(6, cols, device="cuda")
+    w = torch.randn(5, cols, device="cuda")
+    wb = F.quantize_fp8_blocks(w, 128)
+    neg = torch._neg_view(x)
+    imag = torch.complex(w[:, :1].expand(5, cols).contiguous(), w).conj().imag
+    assert neg.is_neg() and imag.is_neg()
+    assert torch.equal(F.quantize_fp8_blocks(neg).q, F.quantize_fp8_blocks(-x).q)
+    assert torch.equal(F.quantize_fp8_blocks(imag).q, F.quantize_fp8_blocks(-w).q)
+    assert torch.equal(F.linear_fp8_blocks(neg, imag), F.linear_fp8_blocks(-x, -w))
+    assert torch.equal(F.linear_fp8_blocks(neg, wb), F.linear_fp8_blocks(-x, wb))
+    assert torch.equal(F.layer_norm(neg), F.layer_norm(-x))
+    v = torch._neg_view(torch.randn(cols, device="cuda"))
+    for call in (lambda: F.layer_norm(x, v), lambda: F.layer_norm(x, None, v),
+                 lambda: F.linear_fp8_blocks(x, w, torch._neg_view(w[:, 0].contiguous()))):
+        with pytest.raises(RuntimeError):
+            call()
+    # a gradient that is one
+    x.requires_grad_()
+    for f in (lambda: F.layer_norm(x), lambda: F.linear_fp8_blocks(x, w)):
+        y = f()
+        dy = torch.randn_like(y)
+        (got,) = torch.autograd.grad(f(), x, torch._neg_view(dy))
+        (want,) = torch.autograd.grad(y, x, -dy)
+        assert torch.equal(got, want)
