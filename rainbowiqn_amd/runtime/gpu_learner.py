@@ -26,6 +26,7 @@ from ..ops.flat_params import (FusedAdam, FusedAdamMixed, attach_flat_grads,
                                flatten_module, master_state_dict)
 from ..ops.functional import quantile_huber_loss_fused
 from ..replay.gpu_replay import GpuReplay
+from .streams import own_stream
 
 
 def _noisy_layers(net: RainbowIQN):
@@ -107,7 +108,7 @@ class GpuLearner:
         # a stream of its own: the math libraries keep one workspace a stream,
         # and graphs captured on the same one would share it.  This one replays
         # beside the actors'.
-        self.capture_stream = torch.cuda.Stream(self.device)
+        self.capture_stream = own_stream(self.device)
         self.steps_per_replay = 1
         self.grad_steps = 0
         # fused no-grad forwards (double-Q select + target quantiles): 4

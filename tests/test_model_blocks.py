@@ -339,3 +339,24 @@ def test_negated_views(cols):
         (got,) = torch.autograd.grad(f(), x, torch._neg_view(dy))
         (want,) = torch.autograd.grad(y, x, -dy)
         assert torch.equal(got, want)
+
+
+@gpu
+def test_capture_streams_are_none_of_torchs():
+    """torch deals out 32 streams in turn: any of them may be another's."""
+    from rainbowiqn_amd.parallel.apex import ApexRunner
+    from rainbowiqn_amd.parallel.comm import Communicator
+
+    pool = {torch.cuda.Stream().cuda_stream for _ in range(40)}
+    cfg = Config(device="cuda", dtype="bf16", learn_start=256, memory_capacity=8192,
+                 learn_per_round=2, cu_split=0, nb_actor=2, **BOTH)
+    runner = ApexRunner(cfg, Communicator(backend="auto"), n_envs=32, chunk_steps=8)
+    used = [runner.glearner] + list(runner.gactors)
+    own = {g.capture_stream.cuda_stream for g in used}
+    assert len(used) == 3 and len(own) == 3 and not own & pool and 0 not in own
+    assert all(g.capture_stream.priority == 0 for g in used)
+    for _ in range(4):
+        runner.run_round()
+    torch.cuda.synchronize()
+    assert all(g.graph is not None for g in used)
+    assert all(torch.isfinite(torch.tensor(l)) for l in runner.losses)
