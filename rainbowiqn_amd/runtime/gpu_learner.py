@@ -456,6 +456,7 @@ class GraphedActor:
         )
         self.use_graph = use_graph
         self.graph: Optional[torch.cuda.CUDAGraph] = None
+        self.capture_stream = own_stream(self.device)  # as the learner's
 
     def _body(self):
         # stack_gather-style preprocess: u8 -> model dtype
@@ -488,7 +489,7 @@ class GraphedActor:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        with torch.cuda.graph(g, stream=self.capture_stream):
             self._body()
         self.graph = g
 

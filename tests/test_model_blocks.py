@@ -360,3 +360,30 @@ def test_capture_streams_are_none_of_torchs():
     torch.cuda.synchronize()
     assert all(g.graph is not None for g in used)
     assert all(torch.isfinite(torch.tensor(l)) for l in runner.losses)
+
+
+@gpu
+def test_act_step_is_captured_on_a_stream_of_its_own():
+    """Replays choose the best actions of the frames that lie there, whatever
+    another graph captured since, and the library workspace is not shared."""
+    from rainbowiqn_amd.runtime.gpu_learner import GraphedActor
+
+    cfg = Config(device="cuda", dtype="fp32", num_quantile_samples=8, **BOTH)
+    torch.manual_seed(0)
+    net = RainbowIQN(cfg, 6).cuda().eval()
+    actors = [GraphedActor(cfg, net, 16) for _ in range(2)]
+    own = {a.capture_stream.cuda_stream for a in actors}
+    assert len(own) == 2 and not own & {torch.cuda.Stream().cuda_stream
+                                        for _ in range(40)}
+    for i in range(4):
+        for a in actors:
+            frames = torch.randint(0, 256, a.stack_u8.shape, dtype=torch.uint8)
+            a.stack_u8.copy_(frames.cuda())
+            got = a.act()
+            torch.cuda.synchronize()
+            with torch.no_grad():  # with the taus that the replay drew
+                z, _ = net(a.stack_u8.float() / 255.0, a.K, taus=a.taus)
+            q = z.mean(dim=1)
+            best = q.max(dim=1).values - q.gather(1, got[:, None])[:, 0]
+            # fp32 sums of up to 3136 terms in another order
+            assert bool((best <= 1e-4 * q.abs().amax()).all())
