@@ -563,7 +563,7 @@ Tensor linear_fp8_serve(Tensor x0, Tensor wq, Tensor ws, int64_t block_rows,
     type_code(x.scalar_type(), "x");
     c10::cuda::CUDAGuard guard(x.device());
     Tensor y = fresh({x.size(0), w.rows}, x.options());
-    if (y.numel() > 0 && riqn_fp8_few(x.size(0), (int)x.size(1)))
+    if (y.numel() > 0 && riqn_fp8_few(x.size(0), w.rows, (int)x.size(1)))
         launched(riqn_fp8_gemm_from(
                      x.data_ptr(), type_code(x.scalar_type(), "x"), x.stride(0),
                      w.q.data_ptr<uint8_t>(), w.scale.data_ptr<uint8_t>(),

@@ -1305,6 +1305,10 @@ __global__ __launch_bounds__(256) void add_shares_kernel(
         default: { using T = fp16_t; __VA_ARGS__; } break; \
     }
 
+// workgroups of 512 threads in a grid's first dimension, which holds less than
+// 2^32 threads
+constexpr int64_t MOST_512 = (1 << 23) - 1;
+
 bool vec8(const void* p, int64_t ld, int C, int type) {
     const int size = type == 0 ? 4 : 2;
     return ((uintptr_t)p & 15) == 0 && (ld * size & 15) == 0 && (C & 7) == 0;
@@ -1376,7 +1380,10 @@ int riqn_fp8_quant_both(const void* x, int64_t ldx, uint8_t* xq, uint8_t* xs,
                         int groups, int M, const void* w, int64_t ldw,
                         uint8_t* wq, uint8_t* ws, uint8_t* wtq, uint8_t* wts,
                         int N, int C, int type, void* stream) {
-    if (!vec8(x, ldx, C, type) || !vec8(w, ldw, C, type)) {
+    const int nb = (C + 127) >> 7, strips = nb >= 4 ? (nb + 3) / 4 : nb;
+    const int64_t tiles = (int64_t)nb * ((N + 127) >> 7);
+    if (!vec8(x, ldx, C, type) || !vec8(w, ldw, C, type) ||
+        tiles + strips > MOST_512) {
         const int err = riqn_fp8_quant_rows(x, type, ldx, nullptr, xq, xs,
                                             nullptr, groups, M, C, stream);
         return err ? err
@@ -1384,21 +1391,20 @@ int riqn_fp8_quant_both(const void* x, int64_t ldx, uint8_t* xq, uint8_t* xs,
                                           stream);
     }
     const Tiles a = tiles_of(w, ldw, wq, ws, wtq, wts, N, C);
-    const bool wide = a.nb >= 4;
-    const int tiles = a.nb * a.nbt, strips = wide ? (a.nb + 3) / 4 : a.nb;
-    const int half = (groups + 1) / 2;  // 8 waves here, 4 there
+    // 8 waves here, 4 there
+    const int half =
+        (int)min((int64_t)(groups + 1) / 2, (MOST_512 - tiles) / strips);
+    const dim3 grid((uint32_t)(tiles + strips * half));
     hipStream_t st = (hipStream_t)stream;
     RIQN_TYPE(type, T, {
-        if (wide)
-            hipLaunchKernelGGL((quant_both_kernel<T, 4>),
-                               dim3(tiles + strips * half), dim3(512), 0, st, a,
-                               (const T*)x, ldx, xq, xs, M, a.nb, a.S, tiles,
-                               strips, half);
+        if (nb >= 4)
+            hipLaunchKernelGGL((quant_both_kernel<T, 4>), grid, dim3(512), 0, st,
+                               a, (const T*)x, ldx, xq, xs, M, nb, a.S,
+                               (int)tiles, strips, half);
         else
-            hipLaunchKernelGGL((quant_both_kernel<T, 1>),
-                               dim3(tiles + strips * half), dim3(512), 0, st, a,
-                               (const T*)x, ldx, xq, xs, M, a.nb, a.S, tiles,
-                               strips, half);
+            hipLaunchKernelGGL((quant_both_kernel<T, 1>), grid, dim3(512), 0, st,
+                               a, (const T*)x, ldx, xq, xs, M, nb, a.S,
+                               (int)tiles, strips, half);
     })
     return (int)hipGetLastError();
 }
@@ -1448,7 +1454,7 @@ int riqn_fp8_gemm(const uint8_t* a, const uint8_t* as, int a_block_rows,
     //      16384           |         | 91 /    | 61 /    | 52 / 89
     // and [30000, 64, 512]:   6 /  8 |  6 /  8 |  7 / 10 | 11 / 17
     RIQN_TYPE(c_type, T, {
-        if (M <= 16) {
+        if (M <= 16 && (N + 15) / 16 <= MOST_512) {
             hipLaunchKernelGGL((gemm_direct_kernel<1, 1, T>),
                                dim3((N + 15) / 16), dim3(512), 0, st, g);
         } else if (tiles(256) >= 192) {
@@ -1473,8 +1479,8 @@ static int few_bytes(int64_t M, int K) {
 }
 
 // whether a product of M rows that are not in 8 bits goes by one kernel
-int riqn_fp8_few(int64_t M, int K) {
-    return M <= 16 && few_bytes(M, K) <= 65536;
+int riqn_fp8_few(int64_t M, int64_t N, int K) {
+    return M <= 16 && few_bytes(M, K) <= 65536 && (N + 15) / 16 <= MOST_512;
 }
 
 // the product of a few rows that are not in 8 bits yet; c has x's type

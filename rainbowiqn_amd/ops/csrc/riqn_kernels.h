@@ -175,7 +175,7 @@ int riqn_fp8_gemm(const uint8_t* a, const uint8_t* as, int a_block_rows,
                   const void* bias, int bias_type, int relu, void* c,
                   int c_type, uint8_t* mask, int exact, int M, int N, int K,
                   void* stream);
-int riqn_fp8_few(int64_t M, int K);
+int riqn_fp8_few(int64_t M, int64_t N, int K);
 int riqn_fp8_gemm_from(const void* x, int type, int64_t ldx, const uint8_t* b,
                        const uint8_t* bs, int b_block_rows, const void* bias,
                        int bias_type, int relu, void* c, int M, int N, int K,

@@ -888,3 +888,34 @@ def test_tangents_cpu():
 @gpu
 def test_tangents_gpu():
     tangents("cuda")
+
+
+@gpu
+def test_more_than_2_32_threads_of_rows():
+    """x of 2^18 rows and 2^17 columns beside the weight in one launch: whole
+    numbers, so every sum is exact (49 x 2^17 is under 2^24, and dw is one row
+    2^18 times)."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randint(-7, 8, (1, 2 ** 17), generator=g).float().cuda()
+    w = torch.randint(-7, 8, (1, 2 ** 17), generator=g).float().cuda().requires_grad_()
+    y = F.linear_fp8_blocks(x.expand(2 ** 18, 2 ** 17), w)
+    assert torch.equal(y, (x.double() @ w.detach().double().t()).float().expand_as(y))
+    (dw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert torch.equal(dw, x * 2 ** 18)
+
+
+@gpu
+def test_more_than_2_32_threads_of_outputs():
+    """One row against 2^27 and more, which the kernels of few rows share out
+    over 512 threads for 16."""
+    n = 2 ** 27 + 5
+    codes = torch.arange(16.0).to(torch.float8_e4m3fn).view(torch.uint8).cuda()
+    q = torch.zeros(n, 128, dtype=torch.uint8, device="cuda")
+    value = torch.arange(n, device="cuda") % 16
+    q[:, 0] = codes[value]
+    w = Fp8Blocks(q, torch.full((n, 4), 127, dtype=torch.uint8, device="cuda"), 3, 1)
+    x = torch.tensor([[3.0, 1.0, -2.0]], device="cuda")
+    want = (3 * value).float()[None]
+    assert torch.equal(F.linear_fp8_blocks(x, w), want)
+    assert torch.equal(F.matmul_fp8_blocks(F.quantize_fp8_blocks(x), w,
+                                           out_dtype=torch.float32), want)
