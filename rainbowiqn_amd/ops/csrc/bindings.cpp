@@ -204,16 +204,6 @@ int64_t create_cu_masked_stream(std::vector<int64_t> mask_words) {
     return (int64_t)(uintptr_t)s;
 }
 
-// A stream of one's own, at the default priority: torch deals its pool of 32
-// out in turn, and what is keyed by stream is then shared.
-int64_t create_stream() {
-    hipStream_t s = nullptr;
-    auto err = hipStreamCreateWithFlags(&s, hipStreamNonBlocking);
-    TORCH_CHECK(err == hipSuccess, "hipStreamCreateWithFlags failed: ",
-                hipGetErrorString(err));
-    return (int64_t)(uintptr_t)s;
-}
-
 void destroy_stream(int64_t ptr) {
     if (ptr) hipStreamDestroy((hipStream_t)(uintptr_t)ptr);
 }
@@ -607,7 +597,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("max_episode_frames"), py::arg("chunk_frames"),
           py::arg("chunk_meta"), py::arg("chunk_pos"), py::arg("task") = 0);
     m.def("create_cu_masked_stream", &create_cu_masked_stream);
-    m.def("create_stream", &create_stream);
     m.def("destroy_stream", &destroy_stream);
     m.def("adam_step_mixed", &adam_step_mixed);
     m.def("noisy_material", &noisy_material);

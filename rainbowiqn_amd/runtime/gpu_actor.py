@@ -18,7 +18,7 @@ import torch
 
 from ..models.model import RainbowIQN
 from ..ops import get_extension
-from .streams import own_stream
+from .streams import capture_stream
 
 FRAME_PX = 84 * 84
 
@@ -70,7 +70,7 @@ class GpuActorLoop:
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         # its own, as graphs of one capture stream share the math libraries'
         # workspace, and this one replays beside the learner's
-        self.capture_stream = own_stream(d)
+        self.capture_stream = capture_stream(self, d)
         self.total_steps = 0
         self._newest = 0  # ring slot of the most recent frame (round-invariant)
         # hand-written fused forward (4 kernels/step) on the bf16 path

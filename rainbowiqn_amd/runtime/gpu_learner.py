@@ -26,7 +26,7 @@ from ..ops.flat_params import (FusedAdam, FusedAdamMixed, attach_flat_grads,
                                flatten_module, master_state_dict)
 from ..ops.functional import quantile_huber_loss_fused
 from ..replay.gpu_replay import GpuReplay
-from .streams import own_stream
+from .streams import capture_stream
 
 
 def _noisy_layers(net: RainbowIQN):
@@ -108,7 +108,7 @@ class GpuLearner:
         # a stream of its own: the math libraries keep one workspace a stream,
         # and graphs captured on the same one would share it.  This one replays
         # beside the actors'.
-        self.capture_stream = own_stream(self.device)
+        self.capture_stream = capture_stream(self, self.device)
         self.steps_per_replay = 1
         self.grad_steps = 0
         # fused no-grad forwards (double-Q select + target quantiles): 4
@@ -456,7 +456,7 @@ class GraphedActor:
         )
         self.use_graph = use_graph
         self.graph: Optional[torch.cuda.CUDAGraph] = None
-        self.capture_stream = own_stream(self.device)  # as the learner's
+        self.capture_stream = capture_stream(self, self.device)  # as the learner's
 
     def _body(self):
         # stack_gather-style preprocess: u8 -> model dtype

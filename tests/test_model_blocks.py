@@ -342,24 +342,47 @@ def test_negated_views(cols):
 
 
 @gpu
-def test_capture_streams_are_none_of_torchs():
+def test_capture_streams_are_apart():
     """torch deals out 32 streams in turn: any of them may be another's."""
     from rainbowiqn_amd.parallel.apex import ApexRunner
     from rainbowiqn_amd.parallel.comm import Communicator
+    from rainbowiqn_amd.runtime import streams
 
-    pool = {torch.cuda.Stream().cuda_stream for _ in range(40)}
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):  # torch's own is there then
+        torch.zeros(1, device="cuda")
+
+    class Owner:
+        def __init__(self):
+            self.stream = streams.capture_stream(self, "cuda")
+
+    first = Owner()
+    for _ in range(40):
+        torch.cuda.Stream()
+        other = Owner()
+        assert other.stream not in (first.stream,
+                                    torch.cuda.graph.default_capture_stream)
+        assert other.stream.priority == 0
+    del first, other
     cfg = Config(device="cuda", dtype="bf16", learn_start=256, memory_capacity=8192,
                  learn_per_round=2, cu_split=0, nb_actor=2, **BOTH)
     runner = ApexRunner(cfg, Communicator(backend="auto"), n_envs=32, chunk_steps=8)
     used = [runner.glearner] + list(runner.gactors)
-    own = {g.capture_stream.cuda_stream for g in used}
-    assert len(used) == 3 and len(own) == 3 and not own & pool and 0 not in own
-    assert all(g.capture_stream.priority == 0 for g in used)
+    own = {g.capture_stream for g in used}
+    own.add(torch.cuda.graph.default_capture_stream)
+    assert len(used) == 3 and len(own) == 4
     for _ in range(4):
         runner.run_round()
     torch.cuda.synchronize()
     assert all(g.graph is not None for g in used)
     assert all(torch.isfinite(torch.tensor(l)) for l in runner.losses)
+    # all of them held, then one given back
+    held = []
+    with pytest.raises(RuntimeError, match="hold all"):
+        for _ in range(streams.POOL):
+            held.append(Owner())
+    assert len(held) <= streams.POOL - 4
+    back = held.pop().stream.cuda_stream
+    assert Owner().stream.cuda_stream == back
 
 
 @gpu
@@ -372,9 +395,7 @@ def test_act_step_is_captured_on_a_stream_of_its_own():
     torch.manual_seed(0)
     net = RainbowIQN(cfg, 6).cuda().eval()
     actors = [GraphedActor(cfg, net, 16) for _ in range(2)]
-    own = {a.capture_stream.cuda_stream for a in actors}
-    assert len(own) == 2 and not own & {torch.cuda.Stream().cuda_stream
-                                        for _ in range(40)}
+    assert len({a.capture_stream for a in actors}) == 2
     for i in range(4):
         for a in actors:
             frames = torch.randint(0, 256, a.stack_u8.shape, dtype=torch.uint8)
