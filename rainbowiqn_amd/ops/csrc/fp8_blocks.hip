@@ -261,7 +261,7 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(
 // be null) get the transposed matrix, whose blocks have the same scales.  One
 // workgroup per block: 32 values a thread stay in registers between the
 // maximum and the conversion; the transposed bytes go through LDS.  Bound by
-// the launch at the sizes of a layer's weight.
+// the launch at the sizes of a layer's weight: [1024, 3136] in bf16 takes 4.4 us.
 // ---------------------------------------------------------------------------
 struct Tiles {
     const void* x;           // [R, C] of T, rows ldx apart
@@ -646,9 +646,9 @@ __global__ __launch_bounds__(512) void gemm_few_kernel(Gemm g) {
 // EXACT: operands expanded to bf16, every product summed in full.  Otherwise
 // the scaled 8-bit instruction, at twice the rate.
 //
-// 256 x 256, 8 waves of 128 x 64: 8192^3 in 457 us (2406 TF) and exact in 789
-// (1393 TF); [32768, 1024, 3136] in 107 to 118 and 182, [32768, 3136, 1024] in
-// 162 and 242, where results are written for as long as two of a tile's 8 steps
+// 256 x 256, 8 waves of 128 x 64, to bf16: 8192^3 exact in 766 us (1436 TF) and
+// scaled in 451 (2440 TF); [32768, 1024, 3136] in 160 to 183 and 102 to 118,
+// [32768, 3136, 1024] in 224 to 252 and 155 to 171, where results are written for as long as two of a tile's 8 steps
 // take.  Products are under way 53 % of the time (8 bits): a step's reads from
 // LDS and its loads into it need as long as they do.  Two groups of waves that
 // read and multiply by turns took 504 us for 8192^3, 4 waves of 128 x 128 more
@@ -943,8 +943,8 @@ void launch_tiles(const Gemm& g, bool exact, hipStream_t st) {
 // products one behind the other.  One tile of 64 x 64 a workgroup; two groups
 // of 4 waves take every other step, so that there are half as many barriers and
 // one group's reads go on under the other's products.  Their sums are added at
-// the end, through LDS.  [1024, 1024, 3136]: 9.3 us in bf16, 13.7 in fp32; with
-// one group 11.9 and 16.0, with four 9.7 and 13.4.
+// the end, through LDS.  [1024, 1024, 3136]: scaled 9.3 us, exact in fp32 13.7;
+// with one group 11.9 and 16.0, with four 9.7 and 13.4.
 template <bool EXACT, typename T>
 __global__ __launch_bounds__(512) void gemm_shared_kernel(Gemm g) {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -1444,7 +1444,7 @@ int riqn_fp8_gemm(const uint8_t* a, const uint8_t* as, int a_block_rows,
     // The largest tile of which there are enough for the 256 CUs: it moves the
     // fewest bytes.  Tiles of 64 that all fit at once, two on a CU, share their
     // steps out over two groups of waves.  Measured in us, scaled products in
-    // bf16 / exact ones in fp32, tiles of 32 (direct) | 64 shared | 64 | 128 | 256; [M, 1024, 3136]:
+    // bf16 / exact ones in fp32 (in bf16 2 to 6 % less), tiles of 32 (direct) | 64 shared | 64 | 128 | 256; [M, 1024, 3136]:
     //   M =  256    9 /  9 |  9 / 13 | 12 / 15 | 19 / 29 | 43 / 74
     //       1024   30 /    |  9 / 14 | 12 / 16 | 20 / 30 | 44 / 75
     //       2048           | 14 / 21 | 18 / 22 | 23 / 31 | 44 / 76

@@ -13,11 +13,12 @@
 // Both passes are bound by memory: forward reads x and writes y, backward
 // reads x and dy and writes dx.  Rows of up to 4096 columns stay in registers
 // between the sums and the result, 8 neighbours a lane and NV times that, so
-// they are read once: [32768, 3136] in bf16 takes 83 us forward (4.9 TB/s) and
-// 136 backward (4.5 TB/s).  A team of 1 wave (up to 1024 columns) or 4 waves takes
+// they are read once: [32768, 3136] in bf16 takes 79 to 85 us forward (4.8 TB/s
+// and more), 139 to 143 backward and 5 to add up the parts (4.2 TB/s).  A team of 1 wave (up to 1024 columns) or 4 waves takes
 // 4 rows at a time: 4 rows of loads in flight, one exchange of sums through
 // LDS for all of them, and the weights stay in registers for the next 4.
-// Longer rows are walked over again by a workgroup, out of the cache.
+// Longer rows are walked over again by a workgroup, value by value: [8192, 8192]
+// in bf16 takes 177 us forward (1.5 TB/s) and 373 backward.
 //
 // dw and db: a lane adds its columns up in registers over all its rows,
 // workgroup g writes part[g], and a second kernel adds the parts.  No atomics:
@@ -71,8 +72,9 @@ struct Pack8 {
 // VEC: rows are 16-byte aligned and C is a multiple of 8; behind column C the
 // values are then zeros where ZERO is set.  Otherwise the last lane takes some
 // columns that the lane before it has too: `fresh` says which count.  Both store
-// the same values for them.  [20001, 2999] in bf16 takes 138 us a step, with the
-// last columns one by one, in a branch, 273.
+// the same values for them.  [20001, 2999] in bf16 takes 133 us a step, with the
+// last columns one by one, in a branch, 273.  A weight that alone lies off 16
+// bytes costs nothing: [32768, 3136] takes 207 us a step, aligned 208.
 template <typename T, bool VEC, bool ZERO>
 DEV Pack8<T> load8(const T* p, int col, int C) {
     Pack8<T> v;
@@ -327,8 +329,8 @@ struct NormBwd {
 };
 
 // 2 waves a SIMD: held to 3 the compiler spills, and [32768, 3136] in bf16
-// takes 165 us instead of 136 with the adding up of the parts (the bytes
-// alone take 121 at the rate of a large copy).
+// took 165 us, the adding up of the parts included, where it takes 144 to 148
+// (the bytes alone take 121 at the rate of a large copy).
 template <typename T, typename W, int TW, int NV, bool VEC>
 __global__ __launch_bounds__(256, 2) void norm_bwd_kernel(NormBwd a) {
     constexpr int TEAMS = 4 / TW;
