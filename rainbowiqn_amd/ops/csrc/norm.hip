@@ -302,7 +302,8 @@ __global__ __launch_bounds__(256) void norm_fwd_long_kernel(NormFwd a) {
             q += d * d;
         });
         const float off = s / a.C, mean = near + off;
-        const float var = s2 / a.C - off * off;
+        // squares past fp32's range leave an infinite variance, not inf - inf
+        const float var = s2 < __builtin_inff() ? s2 / a.C - off * off : s2;
         // rounding may leave less than nothing; a NaN stays one
         const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + a.eps);
         if (a.mean && threadIdx.x == 0) {

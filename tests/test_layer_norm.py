@@ -506,3 +506,23 @@ def test_tangents_cpu():
         for i, call, args in duals(x, w, b):
             got = forward_ad.unpack_dual(call(*args)).tangent
             assert bool(((got.expand_as(h).double() - want[i]).abs() <= 1e-5).all())
+
+
+@gpu
+@pytest.mark.parametrize("cols", [64, 3136, 4100, 40000])
+def test_variances_past_the_range(cols):
+    """Squares past fp32's range make the variance infinite and h zero, as in the
+    plain form in fp32: y is the bias and nothing comes back but the bias's
+    gradient."""
+    x = 1e32 * (1 + torch.rand(3, cols, device="cuda"))
+    x[1, ::2] *= -1
+    x.requires_grad_()
+    w = torch.randn(cols, device="cuda", requires_grad=True)
+    b = torch.randn(cols, device="cuda", requires_grad=True)
+    y = F.layer_norm(x, w, b)
+    assert torch.equal(y, b.detach().expand_as(y))
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    assert not dx.any() and not dw.any() and torch.equal(db, torch.full_like(db, 3.0))
+    # one number in every place: y stays finite, however far the mean is off
+    const = torch.full((1, cols), 1e32, device="cuda")
+    assert F.layer_norm(const, w, b).isfinite().all()
